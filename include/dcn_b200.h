@@ -138,6 +138,13 @@ extern "C" {
 #define DCN_STATUS_FWD_WAIT_TIMEOUT 0x1 /* forward (fwd_tc)                */
 #define DCN_STATUS_BWD_DATA_TIMEOUT 0x2 /* grad-column kernel (bwd_data_tc) */
 #define DCN_STATUS_BWD_WEIGHT_TIMEOUT 0x4 /* weight-gradient kernels        */
+#define DCN_STATUS_DENSE_TIMEOUT 0x8 /* products of the updates and of 8-bit codes */
+
+/* Element types of the entry points that take several. */
+#define DCN_TYPE_F32 0
+#define DCN_TYPE_BF16 1
+#define DCN_TYPE_F16 2
+#define DCN_TYPE_I8 3
 
 /* Geometry of one deformable convolution: the shapes of the reference op's
  * tensors plus its integer arguments. */
@@ -316,6 +323,78 @@ DCN_API size_t dcn_staged_input_size_h16(const dcn_shape* shape);
 DCN_API int dcn_stage_input_h16(const dcn_shape* shape, const void* input, void* staged,
                                 uint32_t flags, void* stream);
 DCN_API int dcn_h16_staging(const dcn_shape* shape, uint32_t flags);
+
+/* Orthogonalised updates (no reference counterpart).  `count` dense matrices
+ * (rows, cols) one after another, of `type`; each becomes `steps` steps of
+ *   X <- a X + (b S + c S S) X,  S = X X^T (X^T X when rows > cols)
+ * from X = G / (|G| + eps), |G| the Frobenius norm; `coefficients` are host
+ * memory: (a, b, c) of each step.  `output` may be `input`.  The products run
+ * on the tensor cores: float32 matrices keep fp32 accuracy (two fp16 terms an
+ * operand), or that of one TF32 product with DCN_MATH_TF32 in `flags`; 16-bit
+ * matrices keep what their type can hold.  A matrix with NaN or an infinity
+ * gives NaN everywhere.  At most 32 steps, 2^31 - 1 elements and a smaller
+ * side of 32768. */
+DCN_API size_t dcn_newton_schulz_workspace_size(int64_t count, int64_t rows, int64_t cols,
+                                                int type, int steps, uint32_t flags);
+DCN_API int dcn_newton_schulz(int64_t count, int64_t rows, int64_t cols, int type,
+                              const void* input, void* output, int steps,
+                              const float* coefficients, float eps, uint32_t flags,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* The optimiser step around it (no reference counterpart), for `count`
+ * matrices of one shape, given as host arrays of device pointers: with m the
+ * float32 momentum,
+ *   m <- momentum m + (1 - momentum) g
+ *   u  = nesterov ? (1 - momentum) g + momentum m : m
+ *   p <- (1 - lr weight_decay) p - lr update_scale orthogonalised(u)
+ * params and grads are of `type`, dense; nothing may overlap.  float32
+ * parameters take DCN_MATH_TF32 as above; 16-bit ones one fp16 product. */
+DCN_API size_t dcn_muon_update_workspace_size(int64_t count, int64_t rows, int64_t cols, int type,
+                                              int steps, uint32_t flags);
+DCN_API int dcn_muon_update(int64_t count, int64_t rows, int64_t cols, int type,
+                            void* const* params, const void* const* grads, float* const* momenta,
+                            float lr, float momentum, int nesterov, float weight_decay,
+                            float update_scale, int steps, const float* coefficients, float eps,
+                            uint32_t flags, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* 8-bit codes of dense rows (no reference counterpart): scale = max |x| / 127
+ * of the row, code = x / scale rounded to the nearest whole number, ties to
+ * even; a row of zeros gets scale 0 and codes 0.  A row with NaN or an
+ * infinity gets that as its scale and codes 0 (its products are NaN). */
+DCN_API int dcn_quantize_int8(int64_t rows, int64_t cols, int type, const void* input,
+                              int8_t* codes, float* scale, void* stream);
+
+/* Products of 8-bit codes with a scale for each token and each output channel
+ * (no reference counterpart): x (tokens, in), weight (out, in), output
+ * (tokens, out), all dense:
+ *   output = (sum_k x weight) x_scale[token] weight_scale[channel] + bias,
+ * the sum exact.  x is int8 with its scales, or floating (x_scale NULL) and
+ * coded as by dcn_quantize_int8 inside the call.  At most 131071 input
+ * features.  Rows of a multiple of 16 features at 16-byte aligned addresses
+ * are read where they lie; others are copied first. */
+DCN_API size_t dcn_int8_linear_workspace_size(int64_t tokens, int64_t in_features,
+                                              int64_t out_features, int x_type);
+DCN_API int dcn_int8_linear(int64_t tokens, int64_t in_features, int64_t out_features, int x_type,
+                            const void* x, const float* x_scale, const int8_t* weight,
+                            const float* weight_scale, const void* bias, int bias_type,
+                            void* output, int out_type, uint32_t flags, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Deformable convolution on such products (forward only; no reference
+ * counterpart).  input, offset and mask of `type` as in dcn_forward; weight
+ * int8 in (outC, kh, kw, C/groups) order, a scale for each output channel
+ * (rows of a multiple of 16 codes at a 16-byte aligned address are read where
+ * they lie, others are copied first).  The sampled columns of each output pixel and group are
+ * coded as by dcn_quantize_int8 (a token), their products with the weight
+ * scaled back.  `flags`: DCN_MASK_LOGITS, DCN_INPUT_NHWC.  The output is dense
+ * NCHW of `out_type`. */
+DCN_API size_t dcn_deform_int8_workspace_size(const dcn_shape* shape, int type, uint32_t flags);
+DCN_API int dcn_deform_int8(const dcn_shape* shape, int type, const void* input,
+                            const int8_t* weight, const float* weight_scale, const void* offset,
+                            const void* mask, const void* bias, int bias_type, void* output,
+                            int out_type, uint32_t flags, void* workspace, size_t workspace_bytes,
+                            void* stream);
 
 /* Device error word of the current device (DCN_STATUS_* bits; 0 when every
  * wait of the tensor-core kernels completed in time).  No reference

@@ -3,7 +3,8 @@
 * ``lib/libdcn_b200.so`` -- the CUDA library (all kernels + the C ABI of
   ``include/dcn_b200.h``), compiled by nvcc for sm_100a only;
 * ``lib/libdcn_b200_torch.so`` -- the PyTorch operator registration
-  (``csrc/torch_ops.cpp``), linked against the library above.
+  (``csrc/torch_ops.cpp``, ``csrc/torch_dense_ops.cpp``), linked against the
+  library above.
 
 Run ``python -m pytorch_mps_deform_conv2d_b200._build`` (or
 ``__graft_entry__.build()``).  Objects are rebuilt only when a source or
@@ -88,10 +89,10 @@ def build_library(verbose: bool = False, force: bool = False) -> str:
 
 
 def build_torch_ops(verbose: bool = False, force: bool = False) -> str:
-    """Compile ``csrc/torch_ops.cpp`` against PyTorch into ``lib/libdcn_b200_torch.so``."""
-    src = os.path.join(CSRC, "torch_ops.cpp")
+    """Compile ``csrc/torch_*.cpp`` against PyTorch into ``lib/libdcn_b200_torch.so``."""
+    srcs = sorted(glob.glob(os.path.join(CSRC, "torch_*.cpp")))
     if (not force and os.path.exists(TORCH_LIB) and
-            os.path.getmtime(TORCH_LIB) >= max(os.path.getmtime(src), os.path.getmtime(LIB),
+            os.path.getmtime(TORCH_LIB) >= max(_newest(srcs), os.path.getmtime(LIB),
                                               _newest(_headers()))):
         return TORCH_LIB
     import torch
@@ -105,14 +106,14 @@ def build_torch_ops(verbose: bool = False, force: bool = False) -> str:
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = (["g++", "-shared", "-fPIC", "-O2", "-std=c++17", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
             "-DTORCH_API_INCLUDE_EXTENSION_H"] + ["-I" + i for i in incs] +
-           [src, "-o", TORCH_LIB, "-L" + torch_lib, "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           srcs + ["-o", TORCH_LIB, "-L" + torch_lib, "-lc10", "-lc10_cuda", "-ltorch_cpu",
             "-ltorch_cuda", "-ltorch", "-L" + os.path.join(cuda, "lib64"), "-lcudart",
             "-L" + LIBDIR, "-ldcn_b200", "-Wl,-rpath,$ORIGIN"])
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"g++ failed on {src}:\n{res.stdout}\n{res.stderr}")
+        raise RuntimeError(f"g++ failed on {srcs}:\n{res.stdout}\n{res.stderr}")
     return TORCH_LIB
 
 

@@ -112,6 +112,29 @@ def load_capi():
         lib.dcn_profiler_read.argtypes = [ctypes.POINTER(KernelStat), ctypes.c_int,
                                           ctypes.POINTER(ctypes.c_int)]
         lib.dcn_profiler_read.restype = ctypes.c_int
+        i32, f32 = ctypes.c_int, ctypes.c_float
+        vpp = ctypes.POINTER(vp)
+        fp = ctypes.POINTER(f32)
+        lib.dcn_newton_schulz_workspace_size.argtypes = [i64] * 3 + [i32, i32, u32]
+        lib.dcn_newton_schulz_workspace_size.restype = sz
+        lib.dcn_newton_schulz.argtypes = [i64] * 3 + [i32, vp, vp, i32, fp, f32, u32, vp, sz, vp]
+        lib.dcn_newton_schulz.restype = i32
+        lib.dcn_muon_update_workspace_size.argtypes = [i64] * 3 + [i32, i32, u32]
+        lib.dcn_muon_update_workspace_size.restype = sz
+        lib.dcn_muon_update.argtypes = ([i64] * 3 + [i32, vpp, vpp, vpp, f32, f32, i32, f32, f32,
+                                                     i32, fp, f32, u32, vp, sz, vp])
+        lib.dcn_muon_update.restype = i32
+        lib.dcn_quantize_int8.argtypes = [i64, i64, i32, vp, vp, vp, vp]
+        lib.dcn_quantize_int8.restype = i32
+        lib.dcn_int8_linear_workspace_size.argtypes = [i64] * 3 + [i32]
+        lib.dcn_int8_linear_workspace_size.restype = sz
+        lib.dcn_int8_linear.argtypes = ([i64] * 3 + [i32, vp, vp, vp, vp, vp, i32, vp, i32, u32,
+                                                     vp, sz, vp])
+        lib.dcn_int8_linear.restype = i32
+        lib.dcn_deform_int8_workspace_size.argtypes = [shp, i32, u32]
+        lib.dcn_deform_int8_workspace_size.restype = sz
+        lib.dcn_deform_int8.argtypes = ([shp, i32] + [vp] * 6 + [i32, vp, i32, u32, vp, sz, vp])
+        lib.dcn_deform_int8.restype = i32
         _capi = lib
         return lib
 

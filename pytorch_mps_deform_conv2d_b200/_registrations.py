@@ -100,6 +100,34 @@ def _col2im_coord_fake(columns, input, offset, mask, kernel_h, kernel_w, stride_
     return offset.new_empty(offset.shape), grad_mask
 
 
+def _newton_schulz_fake(update, steps, coefficients, eps, math=-1):
+    return update.new_empty(update.shape)
+
+
+def _muon_update_fake(params, grads, momenta, lr, momentum, nesterov, weight_decay, steps,
+                      coefficients, eps, match_rms=False, groups=1, math=-1):
+    return None
+
+
+def _quantize_int8_fake(x):
+    return (torch.empty(x.shape, dtype=torch.int8, device=x.device),
+            torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device))
+
+
+def _int8_linear_fake(x, weight, weight_scale, bias=None, x_scale=None, out_dtype=None, flags=0):
+    if out_dtype is None:
+        out_dtype = torch.float32 if x.dtype == torch.int8 else x.dtype
+    return torch.empty(x.shape[:-1] + (weight.shape[0],), dtype=out_dtype, device=x.device)
+
+
+def _deform_conv2d_int8_fake(input, weight, weight_scale, offset, mask, bias, stride_h, stride_w,
+                             pad_h, pad_w, dilation_h, dilation_w, groups, deformable_groups,
+                             out_dtype=None, flags=0):
+    out = _forward_fake(input, weight, offset, mask, bias, stride_h, stride_w, pad_h, pad_w,
+                        dilation_h, dilation_w, groups, deformable_groups)
+    return out if out_dtype is None else out.to(out_dtype)
+
+
 _INT_ARGS = ("stride_h", "stride_w", "pad_h", "pad_w", "dilation_h", "dilation_w", "groups",
              "deformable_groups", "math")
 
@@ -159,3 +187,8 @@ def register() -> None:
     torch.library.register_fake(q + "deform_conv2d_backward_rows")(_backward_rows_fake)
     torch.library.register_autograd(q + "deform_conv2d_forward_rows", _forward_rows_backward,
                                     setup_context=_setup_rows_context)
+    torch.library.register_fake(q + "newton_schulz")(_newton_schulz_fake)
+    torch.library.register_fake(q + "muon_update_")(_muon_update_fake)
+    torch.library.register_fake(q + "quantize_int8")(_quantize_int8_fake)
+    torch.library.register_fake(q + "int8_linear")(_int8_linear_fake)
+    torch.library.register_fake(q + "deform_conv2d_int8")(_deform_conv2d_int8_fake)

@@ -1,0 +1,29 @@
+// dcn_int8.h -- 8-bit codes of rows (a scale each), the sampled columns of a
+// deformable convolution as such rows, and repacking for the products.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "dcn_common.cuh"
+#include "dcn_gemm.h"
+
+namespace dcn {
+
+// x (rows, cols) of `type`, row pitch `ldx` elements -> q (rows, cols) with row
+// pitch `ldq`, scale[row] = max |x| / 127, q = round(x / scale) (ties to even;
+// zeros for a row of zeros).  A row with NaN or an infinity gets zeros and
+// that value as its scale.
+cudaError_t launch_quantize_rows(const void* x, int type, long long rows, int cols, long long ldx,
+                                 signed char* q, long long ldq, float* scale,
+                                 cudaStream_t stream);
+// 8-bit rows into rows of pitch `ldo`.
+cudaError_t launch_repack_i8(const signed char* in, long long rows, int cols, signed char* out,
+                             long long ldo, cudaStream_t stream);
+// Columns of output pixels [p0, p0 + np) (counted over the batch) as 8-bit
+// rows: col[group][pixel - p0][tap * Cg + channel] with row pitch `kp` and
+// scale[group][pixel - p0].  `x` is NHWC; x, offset and mask are of `type`.
+cudaError_t launch_sample_i8(const Geom& g, const void* x, int type, const void* off,
+                             const void* mask, long long p0, int np, signed char* col, int kp,
+                             float* scale, cudaStream_t stream);
+
+}  // namespace dcn

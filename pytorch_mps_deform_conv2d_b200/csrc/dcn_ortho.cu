@@ -1,0 +1,380 @@
+// dcn_ortho.cu -- Newton-Schulz orthogonalisation of a batch of matrices, and
+// the momentum optimiser step that uses it.
+//
+// X <- a X + (b S + c S S) X with S = X X^T, some steps over, starting from
+// G / (|G| + eps).  Each step multiplies X by a polynomial of S, and all those
+// polynomials commute, so a run of steps needs X only at its ends:
+//   S = X X^T;  each step: P = a I + b S + c S S;  Q <- P Q;  S <- P (P S);
+//   then X <- Q X.
+// For m x n with n = 9 m (a layer of 3 x 3 taps) two runs for five steps take
+// 68 m^3 flops of symmetric and plain products, the recurrence as written 140.
+//
+// A run cannot be long.  The rounding of S, 2^-22 of its largest value with
+// two fp16 terms, is a larger relative error of the small singular values'
+// part of it, and every further step of the run multiplies that by a^2 while
+// those values grow.  A run ends before the product of its a^2 passes 150:
+// three steps of the usual 3.4445, two runs for five steps; results of 16 bits
+// do not see the difference.  For fp32 results the first run, where one
+// direction can hold nearly all of |X|, ends before 12: two steps, then three.
+// Emulated in 64 bits on 64 x 576 with a few strong directions, the relative
+// error is 5e-7 with (2, 3) and 4.6e-6 with (3, 2), fp32 products as written
+// 1.4e-6; over flat, power-law and exponential spectra (2, 3) stays within 1.6
+// times fp32 products or below them; one run of five steps diverges.
+#include "dcn_ortho.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "dcn_capi_util.h"
+
+namespace dcn {
+
+namespace {
+
+// Powers of two that bring fp16 into the middle of its range: S (at most 1.5
+// in a run of the usual steps, 8 at most), P (its coefficients, 16 at most),
+// Q (products of at most 150^(1/2) with room for 256).
+constexpr float kScaleS = 8192.f, kScaleP = 4096.f, kScaleQ = 256.f;
+constexpr int kPartials = 64;  // sums of squares a matrix
+constexpr float kRunLimit = 150.f, kFirstRunLimit = 12.f;
+
+struct PrepArgs {
+  const void* in[kGemmMaxList];
+  float* momentum[kGemmMaxList];
+  double* partial;  // [count][kPartials]
+  float* r1;        // [count] true X = r1 * stored X
+  float* r2;        // [count] r1 squared
+  unsigned short* x;
+  long long numel, pitch, term_stride, batch_stride;
+  int rows, cols, type, terms, target;  // |stored X| lies in [2^target, 2^(target + 1))
+  int muon, nesterov;
+  float beta, eps;
+};
+
+__device__ __forceinline__ float load_in(const PrepArgs& a, int b, long long i) {
+  const void* p = a.in[b];
+  if (a.type == kF32) return static_cast<const float*>(p)[i];
+  if (a.type == kBF16T) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+
+// The update's value at i from the new momentum.
+__device__ __forceinline__ float update_of(const PrepArgs& a, float g, float m) {
+  return a.nesterov ? (1.f - a.beta) * g + a.beta * m : m;
+}
+
+// New momentum, and sums of squares of the update in 64 bits: any fp32 input
+// keeps its norm, and the partial sums' fixed order keeps the result.
+__global__ void __launch_bounds__(256) ortho_norm_kernel(const __grid_constant__ PrepArgs a) {
+  const int b = blockIdx.y;
+  double s = 0.0;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.numel;
+       i += (long long)kPartials * 256) {
+    float v = load_in(a, b, i);
+    if (a.muon) {
+      const float m = a.beta * a.momentum[b][i] + (1.f - a.beta) * v;
+      a.momentum[b][i] = m;
+      v = update_of(a, v, m);
+    }
+    s += (double)v * (double)v;
+  }
+  __shared__ double red[8];
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) s += red[w];
+    a.partial[b * kPartials + blockIdx.x] = s;
+  }
+}
+
+// X as fp16 terms of the update times a power of two: exact for 16-bit inputs
+// (but for what lies 2^-24 below the largest), and 1 / (norm + eps) is left to
+// the products' epilogues in fp32.
+__global__ void __launch_bounds__(256) ortho_scale_kernel(const __grid_constant__ PrepArgs a) {
+  const int b = blockIdx.y;
+  __shared__ float f1, f2;
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int i = 0; i < kPartials; ++i) s += a.partial[b * kPartials + i];
+    const double norm = sqrt(s);
+    int k = 0;
+    if (norm > 0.0 && isfinite(norm)) k = a.target - ilogb(norm);
+    f1 = (float)ldexp(1.0, k / 2);
+    f2 = (float)ldexp(1.0, k - k / 2);
+    if (blockIdx.x == 0) {
+      // a norm that is not finite leaves nothing to scale by
+      const float r = isfinite(norm) ? (float)ldexp(1.0 / (norm + (double)a.eps), -k)
+                                     : __int_as_float(0x7fc00000);
+      a.r1[b] = r;
+      a.r2[b] = r * r;
+    }
+  }
+  __syncthreads();
+  const int chunks = (int)(a.pitch / 8);
+  const long long total = (long long)a.rows * chunks;
+  for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < total;
+       q += (long long)gridDim.x * 256) {
+    const int row = (int)(q / chunks), c = (int)(q - (long long)row * chunks) * 8;
+    __align__(16) unsigned short hi[8], lo[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float v = 0.f;
+      if (c + j < a.cols) {
+        const long long i = (long long)row * a.cols + c + j;
+        v = load_in(a, b, i);
+        if (a.muon) v = update_of(a, v, a.momentum[b][i]);
+        v = v * f1 * f2;
+      }
+      const __half h = __float2half_rn(v);
+      hi[j] = __half_as_ushort(h);
+      lo[j] = __half_as_ushort(__float2half_rn(v - __half2float(h)));
+    }
+    unsigned short* x = a.x + (long long)b * a.batch_stride + (long long)row * a.pitch + c;
+    *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(hi);
+    if (a.terms == 2)
+      *reinterpret_cast<uint4*>(x + a.term_stride) = *reinterpret_cast<const uint4*>(lo);
+  }
+}
+
+constexpr size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
+
+struct Layout {
+  int m, n;  // smaller and larger side
+  bool wide;
+  long long xpitch, xterm;  // elements
+  long long spitch, sterm;
+  size_t x_bytes, s_bytes;  // one matrix, both terms of a slot / as many as needed
+  int x_terms;
+  size_t scalars, partials, total;
+};
+
+Layout layout_of(const OrthoShape& s, int count) {
+  Layout l;
+  l.wide = s.rows <= s.cols;
+  l.m = l.wide ? s.rows : s.cols;
+  l.n = l.wide ? s.cols : s.rows;
+  auto up8 = [](long long v) { return (v + 7) / 8 * 8; };
+  l.xpitch = up8(s.cols);
+  l.xterm = l.xpitch * s.rows;
+  l.spitch = up8(l.m);
+  l.sterm = l.spitch * l.m;
+  l.x_terms = s.first_terms > s.later_terms ? s.first_terms : s.later_terms;
+  l.x_bytes = align_up((size_t)count * l.x_terms * l.xterm * 2);
+  l.s_bytes = align_up((size_t)count * 2 * l.sterm * 2);
+  l.partials = align_up((size_t)count * kPartials * sizeof(double));
+  l.scalars = align_up((size_t)count * 2 * sizeof(float));
+  l.total = l.partials + l.scalars + 2 * l.x_bytes + 5 * l.s_bytes;
+  return l;
+}
+
+int run_length(const OrthoShape& s, int first) {
+  // the steps after the first of a run rest on an S that the run itself made
+  const bool f32 = s.first_terms == 2 && s.later_terms == 2;
+  const float limit = first == 0 && f32 ? kFirstRunLimit : kRunLimit;
+  float grown = 1.f;
+  int k = first;
+  while (k + 1 < s.steps) {
+    const float a = s.coef[3 * k];
+    grown *= a * a > 1.f ? a * a : 1.f;
+    if (!(grown <= limit)) break;
+    ++k;
+  }
+  return k + 1 - first;
+}
+
+int log2_floor(double v) {
+  int e = 0;
+  while (v >= 2.0) {
+    v *= 0.5;
+    ++e;
+  }
+  return e;
+}
+
+}  // namespace
+
+size_t ortho_workspace_bytes(const OrthoShape& s, int count) {
+  return layout_of(s, count).total + 256;
+}
+
+cudaError_t launch_ortho(const OrthoShape& s, const OrthoChunk& c, void* workspace,
+                         long long wait_limit, int no_async, cudaStream_t stream,
+                         const char** stage) {
+  const Layout l = layout_of(s, c.count);
+  char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(workspace) + 255) &
+                                     ~(uintptr_t)255);
+  double* partial = reinterpret_cast<double*>(ws);
+  float* r1 = reinterpret_cast<float*>(ws + l.partials);
+  float* r2 = r1 + c.count;
+  char* at = ws + l.partials + l.scalars;
+  auto take = [&](size_t bytes) {
+    unsigned short* p = reinterpret_cast<unsigned short*>(at);
+    at += bytes;
+    return p;
+  };
+  unsigned short* x[2] = {take(l.x_bytes), take(l.x_bytes)};
+  unsigned short *S = take(l.s_bytes), *P = take(l.s_bytes), *C = take(l.s_bytes);
+  unsigned short* Q[2] = {take(l.s_bytes), take(l.s_bytes)};
+
+  // |X| = 1: entries of about 1 on average, and 2^15 at the most
+  const double area = (double)s.rows * s.cols;
+  int target = log2_floor(area) / 2;
+  if (target > 14) target = 14;
+  // between runs |X| is up to sqrt(m), entries about n^-1/2 and 1.5 at the most
+  int later = log2_floor((double)l.n) / 2 + 4;
+  if (later > 14) later = 14;
+  const float later_scale = (float)(1 << later);
+
+  PrepArgs p;
+  for (int i = 0; i < c.count; ++i) {
+    p.in[i] = c.in[i];
+    p.momentum[i] = c.momentum[i];
+  }
+  p.partial = partial;
+  p.r1 = r1;
+  p.r2 = r2;
+  p.x = x[0];
+  p.numel = (long long)s.rows * s.cols;
+  p.pitch = l.xpitch;
+  p.term_stride = l.xterm;
+  p.batch_stride = l.xterm * s.first_terms;
+  p.rows = s.rows;
+  p.cols = s.cols;
+  p.type = s.type;
+  p.terms = s.first_terms;
+  p.target = target;
+  p.muon = c.muon;
+  p.nesterov = c.nesterov;
+  p.beta = c.beta;
+  p.eps = s.eps;
+  *stage = "ortho_norm";
+  capi::ProfScope norm_scope(*stage, stream);
+  ortho_norm_kernel<<<dim3(kPartials, c.count), 256, 0, stream>>>(p);
+  norm_scope.done();
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  *stage = "ortho_scale";
+  const long long chunks = s.rows * (l.xpitch / 8);
+  const long long blocks = (chunks + 255) / 256;
+  capi::ProfScope scale_scope(*stage, stream);
+  ortho_scale_kernel<<<dim3((unsigned)(blocks < 592 ? blocks : 592), c.count), 256, 0, stream>>>(p);
+  scale_scope.done();
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+
+  auto square = [&](const unsigned short* base) {
+    GemmOperand o{base, l.m, l.m, l.spitch, 2, l.sterm, c.count, 2 * l.sterm, false};
+    return o;
+  };
+  auto product = [&](const char* name, const GemmOperand& a, const GemmOperand& b, int M, int N,
+                     int K, GemmEpiArgs epi, bool sym) {
+    GemmProblem g{};
+    g.a = a;
+    g.b = b;
+    g.M = M;
+    g.N = N;
+    g.K = K;
+    g.batch = c.count;
+    g.sym = sym;
+    g.epi = epi;
+    g.wait_limit = wait_limit;
+    g.no_async = no_async;
+    *stage = name;
+    capi::ProfScope scope(name, stream);
+    const cudaError_t err = launch_gemm(g, stream);
+    scope.done();
+    return err;
+  };
+  auto to_square = [&](unsigned short* out, float factor) {
+    GemmEpiArgs q{};
+    q.mode = kEpiTerms;
+    q.factor = factor;
+    q.out16 = out;
+    q.out_terms = 2;
+    q.pitch = l.spitch;
+    q.term_stride = l.sterm;
+    q.batch_stride = 2 * l.sterm;
+    return q;
+  };
+
+  int terms = s.first_terms, cur = 0;
+  for (int k = 0; k < s.steps;) {
+    const int run = run_length(s, k);
+    const bool first = k == 0, last = k + run == s.steps;
+    const GemmOperand X{x[cur], s.rows, s.cols, l.xpitch, terms, l.xterm, c.count,
+                        terms * l.xterm, !l.wide};
+    const float xs = first ? 1.f : 1.f / later_scale;
+    GemmEpiArgs q = to_square(S, xs * xs * kScaleS);
+    if (first) q.scale = r2;
+    e = product("ortho_gram", X, X, l.m, l.m, l.n, q, true);
+    if (e != cudaSuccess) return e;
+    unsigned short* prod = nullptr;  // Q so far
+    for (int i = 0; i < run; ++i) {
+      const float* abc = s.coef + 3 * (k + i);
+      unsigned short* poly = prod == nullptr ? Q[0] : P;
+      const float to = prod == nullptr ? kScaleQ : kScaleP;
+      q = to_square(poly, abc[2] * to / (kScaleS * kScaleS));
+      q.mode = kEpiPoly;
+      q.diag = abc[0] * to;
+      q.lin = abc[1] * to / kScaleS;
+      q.lin16 = S;
+      e = product("ortho_poly", square(S), square(S), l.m, l.m, l.m, q, true);
+      if (e != cudaSuccess) return e;
+      if (i + 1 < run) {  // S <- P (P S)
+        e = product("ortho_square", square(poly), square(S), l.m, l.m, l.m,
+                    to_square(C, 1.f / to), true);
+        if (e != cudaSuccess) return e;
+        e = product("ortho_square", square(poly), square(C), l.m, l.m, l.m,
+                    to_square(S, 1.f / to), true);
+        if (e != cudaSuccess) return e;
+      }
+      if (prod == nullptr) {
+        prod = poly;
+      } else {
+        unsigned short* next = prod == Q[0] ? Q[1] : Q[0];
+        e = product("ortho_chain", square(poly), square(prod), l.m, l.m, l.m,
+                    to_square(next, 1.f / to), true);
+        if (e != cudaSuccess) return e;
+        prod = next;
+      }
+    }
+    GemmEpiArgs o{};
+    o.factor = xs / kScaleQ;
+    if (first) o.scale = r1;
+    if (last) {
+      o.mode = c.muon ? kEpiAxpy : kEpiOut;
+      if (c.muon) {
+        o.factor *= c.step;
+        o.keep = c.keep;
+      }
+      o.out_type = s.type;
+      const int es = s.type == kF32 ? 4 : 2;
+      o.wide_ok = (long long)s.cols * es % 16 == 0;
+      for (int i = 0; i < c.count; ++i) {
+        o.list[i] = c.out[i];
+        if (reinterpret_cast<uintptr_t>(c.out[i]) % 16 != 0) o.wide_ok = 0;
+      }
+    } else {
+      o.mode = kEpiTerms;
+      o.factor *= later_scale;
+      o.out16 = x[cur ^ 1];
+      o.out_terms = s.later_terms;
+      o.pitch = l.xpitch;
+      o.term_stride = l.xterm;
+      o.batch_stride = s.later_terms * l.xterm;
+    }
+    // Q X with X's rows along K, or X Q with X as it lies
+    GemmOperand t = X;
+    t.k_rows = l.wide;
+    e = l.wide ? product("ortho_apply", square(prod), t, l.m, l.n, l.m, o, false)
+               : product("ortho_apply", t, square(prod), l.n, l.m, l.m, o, false);
+    if (e != cudaSuccess) return e;
+    cur ^= 1;
+    terms = s.later_terms;
+    k += run;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace dcn

@@ -84,4 +84,26 @@ cudaError_t make_tmap_2d_h16_box(CUtensorMap* map, const void* base, uint64_t in
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+cudaError_t make_tmap_4d(CUtensorMap* map, const void* base, bool int8, uint64_t inner,
+                         uint64_t rows, uint64_t pitch, uint64_t terms, uint64_t term_stride,
+                         uint64_t batch, uint64_t batch_stride, uint32_t box_rows) {
+  std::call_once(g_encode_once, resolve_encode);
+  if (g_encode_status != cudaSuccess) return g_encode_status;
+  const uint64_t es = int8 ? 1 : 2;
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (pitch * es) % 16 != 0 ||
+      (term_stride * es) % 16 != 0 || (batch_stride * es) % 16 != 0 || box_rows == 0 ||
+      box_rows > 256 || inner == 0 || rows == 0 || terms == 0 || batch == 0)
+    return cudaErrorInvalidValue;
+  const cuuint64_t dims[4] = {inner, rows, terms, batch};
+  const cuuint64_t strides[3] = {pitch * es, term_stride * es, batch_stride * es};
+  const cuuint32_t box[4] = {(cuuint32_t)(128 / es), box_rows, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = g_encode(
+      map, int8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+      const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 }  // namespace dcn

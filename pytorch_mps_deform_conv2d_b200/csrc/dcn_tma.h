@@ -29,4 +29,12 @@ cudaError_t make_tmap_2d_h16_box(CUtensorMap* map, const void* base, uint64_t in
                                  uint64_t rows, uint64_t pitch_elems, uint32_t box_inner,
                                  uint32_t box_rows, bool f16);
 
+// 4-D tensor map over `batch` matrices of `terms` parts of `rows` rows of
+// `inner` contiguous elements (fp16, or 8-bit with `int8`); strides in
+// elements, each a multiple of 16 bytes.  Boxes of 128 bytes x `box_rows` rows
+// of one part of one matrix, 128-byte swizzle, zeros out of range.
+cudaError_t make_tmap_4d(CUtensorMap* map, const void* base, bool int8, uint64_t inner,
+                         uint64_t rows, uint64_t pitch, uint64_t terms, uint64_t term_stride,
+                         uint64_t batch, uint64_t batch_stride, uint32_t box_rows);
+
 }  // namespace dcn

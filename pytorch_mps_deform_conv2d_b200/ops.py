@@ -32,9 +32,11 @@ TEST_WAIT_TIMEOUT = 0x1000000
 STATUS_FWD_WAIT_TIMEOUT = 0x1
 STATUS_BWD_DATA_TIMEOUT = 0x2
 STATUS_BWD_WEIGHT_TIMEOUT = 0x4
+STATUS_DENSE_TIMEOUT = 0x8
 _STATUS_NAMES = {STATUS_FWD_WAIT_TIMEOUT: "forward (fwd_tc)",
                  STATUS_BWD_DATA_TIMEOUT: "grad-column kernel (bwd_data_tc)",
-                 STATUS_BWD_WEIGHT_TIMEOUT: "weight-gradient kernel"}
+                 STATUS_BWD_WEIGHT_TIMEOUT: "weight-gradient kernel",
+                 STATUS_DENSE_TIMEOUT: "matrix products of the updates and of 8-bit codes"}
 
 
 def device_status(clear: bool = True) -> int:

@@ -1,0 +1,136 @@
+"""Host-side behaviour of the orthogonalised updates and 8-bit products: no
+fallback on the CPU, refusals of the C entry points before anything is
+launched, shape inference of the operators."""
+import ctypes
+
+import pytest
+import torch
+
+import pytorch_mps_deform_conv2d_b200 as dcn
+from pytorch_mps_deform_conv2d_b200 import _native
+
+F32, BF16, F16, I8 = range(4)
+OK, INVALID, WORKSPACE, CUDA, UNSUPPORTED = range(5)
+P = 1 << 20  # an address that is never read: every call below is refused on the host
+
+
+def test_cpu_tensors_are_refused():
+    x, q, s = torch.randn(4, 16), torch.zeros(4, 16, dtype=torch.int8), torch.ones(4)
+    for call in (lambda: dcn.newton_schulz(x), lambda: dcn.muon_update_([x], [x], [x], lr=0.1),
+                 lambda: dcn.quantize_int8(x), lambda: dcn.int8_linear(x, q, s),
+                 lambda: dcn.deform_conv2d_int8(torch.randn(1, 2, 5, 5), torch.zeros(1, 18, 3, 3),
+                                                torch.zeros(2, 2, 3, 3, dtype=torch.int8), s[:2])):
+        with pytest.raises(NotImplementedError, match="CUDA"):
+            call()
+
+
+def test_optimizer_arguments():
+    w = torch.nn.Parameter(torch.randn(6, 4))
+    for kw in (dict(lr=-1.0), dict(momentum=1.0), dict(weight_decay=-0.1), dict(adjust="none")):
+        with pytest.raises(ValueError):
+            dcn.Muon([w], **kw)
+    with pytest.raises(ValueError, match="two dimensions"):
+        dcn.Muon([torch.nn.Parameter(torch.randn(6))])
+    with pytest.raises(ValueError, match="divisible"):
+        dcn.Muon([dict(params=[w], groups=4)])
+    opt = dcn.Muon([w])
+    assert opt.step() is None  # nothing has a gradient: nothing is called
+    with pytest.raises(ValueError, match="adjust"):
+        dcn.muon_update_([w], [w], [w], lr=0.1, adjust="x")
+
+
+def coef(*v):
+    return (ctypes.c_float * len(v))(*v)
+
+
+def test_newton_schulz_c_refusals():
+    lib = _native.load_capi()
+    c = coef(3.4, -4.8, 2.0)
+    ws = lib.dcn_newton_schulz_workspace_size(1, 64, 128, F32, 1, 0)
+    assert ws > 0 and lib.dcn_newton_schulz_workspace_size(1, 64, 128, I8, 1, 0) == 0
+    assert lib.dcn_newton_schulz_workspace_size(1, 64, 128, F32, 33, 0) == 0
+
+    def call(count=1, rows=64, cols=128, t=F32, x=P, out=P, steps=1, co=c, eps=0.0, n=ws, w=P):
+        return lib.dcn_newton_schulz(count, rows, cols, t, x, out, steps, co, eps, 0, w, n, None)
+
+    assert call(n=ws - 1) == WORKSPACE and call(w=None) == WORKSPACE
+    assert call(x=None) == INVALID and call(out=None) == INVALID and call(co=None) == INVALID
+    assert call(t=I8) == INVALID and call(steps=0) == INVALID and call(eps=-1.0) == INVALID
+    assert call(rows=-1) == INVALID and call(co=coef(1e9, 0, 0)) == INVALID
+    assert call(rows=1 << 16, cols=1 << 15) == UNSUPPORTED
+    assert call(rows=40000, cols=40000) == UNSUPPORTED
+    assert call(count=0) == OK and call(rows=0) == OK
+    assert b"dcn_newton_schulz" in (call(x=None), lib.dcn_last_error())[1]
+
+
+def test_muon_c_refusals():
+    lib = _native.load_capi()
+    c = coef(3.4, -4.8, 2.0)
+    vp = ctypes.c_void_p
+    some, none = (vp * 1)(P), (vp * 1)(None)
+    ws = lib.dcn_muon_update_workspace_size(1, 64, 128, BF16, 1, 0)
+
+    def call(p=some, g=some, m=some, momentum=0.9, n=ws, t=BF16):
+        return lib.dcn_muon_update(1, 64, 128, t, p, g, m, 0.1, momentum, 1, 0.0, 1.0, 1, c, 1e-7, 0,
+                                   P, n, None)
+
+    assert call(p=none) == INVALID and call(g=none) == INVALID and call(m=none) == INVALID
+    assert call(p=None) == INVALID and call(momentum=1.0) == INVALID and call(t=I8) == INVALID
+    assert call(n=ws - 1) == WORKSPACE
+
+
+def test_int8_c_refusals():
+    lib = _native.load_capi()
+    assert lib.dcn_quantize_int8(2, 8, I8, P, P, P, None) == INVALID
+    assert lib.dcn_quantize_int8(2, 8, F32, None, P, P, None) == INVALID
+    assert lib.dcn_quantize_int8(1 << 31, 8, F32, P, P, P, None) == UNSUPPORTED
+    assert lib.dcn_quantize_int8(0, 8, F32, None, None, None, None) == OK
+    ws = lib.dcn_int8_linear_workspace_size(4, 64, 32, F16)
+    assert ws > 0 and lib.dcn_int8_linear_workspace_size(0, 64, 32, F16) == 0
+
+    def call(tokens=4, cin=64, cout=32, t=F16, x=P, xs=None, w=P, sc=P, b=None, bt=F32, o=P, ot=F16,
+             n=ws):
+        return lib.dcn_int8_linear(tokens, cin, cout, t, x, xs, w, sc, b, bt, o, ot, 0, P, n, None)
+
+    assert call(xs=P) == INVALID and call(t=I8) == INVALID  # x_scale with int8 and only then
+    assert call(x=None) == INVALID and call(w=None) == INVALID and call(sc=None) == INVALID
+    assert call(o=None) == INVALID and call(ot=I8) == INVALID and call(b=P, bt=I8) == INVALID
+    assert call(cin=0) == INVALID and call(cin=131072) == UNSUPPORTED
+    assert call(n=ws - 1) == WORKSPACE and call(tokens=0) == OK
+
+
+def test_deform_int8_c_refusals():
+    lib = _native.load_capi()
+    good = dict(batch=1, in_channels=4, height=6, width=6, out_channels=4, kernel_h=3, kernel_w=3,
+                stride_h=1, stride_w=1, pad_h=1, pad_w=1, dilation_h=1, dilation_w=1, groups=1,
+                deformable_groups=1)
+
+    def call(t=F32, x=P, n=1 << 30, ot=F32, **kw):
+        s = _native.DcnShape(**{**good, **kw})
+        return lib.dcn_deform_int8(ctypes.byref(s), t, x, P, P, P, None, None, F32, P, ot, 0, P, n,
+                                   None)
+
+    assert call(n=16) == WORKSPACE and call(x=None) == INVALID and call(t=I8) == INVALID
+    assert call(ot=I8) == INVALID and call(stride_h=0) == INVALID and call(groups=3) == INVALID
+    assert call(in_channels=20000) == UNSUPPORTED  # 180000 columns a group
+    assert call(batch=0) == OK
+
+
+def meta(*shape, dtype=torch.float32):
+    return torch.empty(*shape, device="meta", dtype=dtype)
+
+
+def test_operators_infer_shapes():
+    ops = _native.load_ops()
+    y = ops.newton_schulz(meta(3, 8, 4, dtype=torch.bfloat16), 5, [1.0, 0.0, 0.0], 1e-7)
+    assert y.shape == (3, 8, 4) and y.dtype == torch.bfloat16
+    q, s = ops.quantize_int8(meta(3, 5, 8))
+    assert q.shape == (3, 5, 8) and q.dtype == torch.int8 and s.shape == (3, 5)
+    w = meta(6, 8, dtype=torch.int8)
+    assert ops.int8_linear(meta(2, 3, 8, dtype=torch.half), w, meta(6)).dtype == torch.half
+    y = ops.int8_linear(meta(2, 8, dtype=torch.int8), w, meta(6), None, meta(2))
+    assert y.shape == (2, 6) and y.dtype == torch.float32
+    y = ops.deform_conv2d_int8(meta(2, 4, 9, 9), meta(6, 4, 3, 3, dtype=torch.int8), meta(6),
+                               meta(2, 18, 9, 9), None, None, 1, 1, 1, 1, 1, 1, 1, 1,
+                               torch.bfloat16)
+    assert y.shape == (2, 6, 9, 9) and y.dtype == torch.bfloat16
