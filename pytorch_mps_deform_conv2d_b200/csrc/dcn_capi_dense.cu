@@ -302,6 +302,14 @@ DCN_API int dcn_int8_linear(int64_t tokens, int64_t in_features, int64_t out_fea
     return fail(DCN_ERR_WORKSPACE, "dcn_int8_linear: workspace too small");
   if (!aligned16(x)) p.pack_x = true;
   if (!aligned16(weight)) p.pack_w = true;
+  if (dcn::few_tokens_fit(tokens, in_features) && aligned16(x) && aligned16(weight)) {
+    DCN_CUDA(dcn::launch_few_tokens(x, x_type, x_scale, (int)tokens, (int)in_features,
+                                    (int)out_features,
+                                    reinterpret_cast<const signed char*>(weight), weight_scale,
+                                    bias, bias_type, output, out_type, stream),
+             "few_tokens");
+    return DCN_OK;
+  }
   Carve ws(workspace);
   signed char* xq = ws.take<signed char>(p.x_bytes);
   float* xs = ws.take<float>(p.scale_bytes);

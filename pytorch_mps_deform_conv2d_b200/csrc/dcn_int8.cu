@@ -55,6 +55,87 @@ quantize_rows_kernel(const void* __restrict__ x, int cols, long long ldx,
     q[row * ldq + c] = (signed char)code_of(ld<T>(x, row * ldx + c), s, ok);
 }
 
+// Eight consecutive values (16-byte aligned) as fp32.
+template <int T>
+__device__ __forceinline__ void ld8(const void* p, long long i, float (&v)[8]) {
+  if constexpr (T == kF32) {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const float4 a = __ldg(q), b = __ldg(q + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    const uint4 r = __ldg(
+        reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(p) + i));
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (T == kBF16T) {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        v[2 * j] = f.x;
+        v[2 * j + 1] = f.y;
+      }
+    }
+  }
+}
+// The codes of eight values, the first in the lowest byte.
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], float s, bool ok) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    w[j >> 2] |= (uint32_t)(code_of(v[j], s, ok) & 255) << (8 * (j & 3));
+  return make_uint2(w[0], w[1]);
+}
+
+// Rows of a multiple of eight values at 16-byte aligned addresses.  A row is
+// read once: the first 8 * 256 * KEEP of its values wait in registers for
+// their scale.  Bound by HBM.
+template <int T>
+__global__ void __launch_bounds__(256)
+quantize_rows8_kernel(const void* __restrict__ x, int vecs, long long ldx,
+                      signed char* __restrict__ q, long long ldq, float* __restrict__ scale) {
+  constexpr int KEEP = 4;
+  const long long row = blockIdx.x;
+  const int tid = threadIdx.x, nt = blockDim.x;
+  float v[KEEP][8];
+  unsigned top = 0;
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k) {
+    const int c = tid + k * nt;
+    if (c < vecs) {
+      ld8<T>(x, row * ldx + 8LL * c, v[k]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[k][j]));
+    }
+  }
+  for (int c = tid + KEEP * nt; c < vecs; c += nt) {
+    float u[8];
+    ld8<T>(x, row * ldx + 8LL * c, u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, abs_bits(u[j]));
+  }
+  __shared__ unsigned red[8];
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((tid & 31) == 0) red[tid >> 5] = top;
+  __syncthreads();
+  for (int w = 0; w < nt / 32; ++w) top = max(top, red[w]);
+  const float s = scale_of(top);
+  const bool ok = usable_scale(s);
+  if (tid == 0) scale[row] = s;
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k) {
+    const int c = tid + k * nt;
+    if (c < vecs) *reinterpret_cast<uint2*>(q + row * ldq + 8LL * c) = codes8(v[k], s, ok);
+  }
+  for (int c = tid + KEEP * nt; c < vecs; c += nt) {
+    float u[8];
+    ld8<T>(x, row * ldx + 8LL * c, u);
+    *reinterpret_cast<uint2*>(q + row * ldq + 8LL * c) = codes8(u, s, ok);
+  }
+}
+
 __global__ void __launch_bounds__(256)
 repack_i8_kernel(const signed char* __restrict__ in, long long rows, int cols,
                  signed char* __restrict__ out, long long ldo) {
@@ -135,11 +216,283 @@ sample_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ of
   if (lane == 0) scale[(long long)gi * np + lp] = s;
 }
 
+// Channels in eights (per group, per deformable group).  WPP warps share an
+// item, so that each lane holds at most NV vectors of eight samples in
+// registers from the gather to their codes: the input is gathered once and
+// only codes are written.  The sampling plans of an item (corner offsets,
+// weights with the mask) are made once, a lane each, in shared memory; then
+// lane l takes vectors l, l + 32 WPP, ... of the column.  Bound by the L2 -> SM
+// traffic of the corners (four of 16 bytes for eight codes).
+struct alignas(16) PlanI8 {
+  int at[4];  // element offsets of the corners within the image
+  float w[4];
+};
+
+template <int T, int NV>
+__global__ void __launch_bounds__(256, NV <= 3 ? 4 : 2)
+sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ off,
+                  const void* __restrict__ mask, long long p0, int np,
+                  signed char* __restrict__ col, int kp, float* __restrict__ scale, int wpp,
+                  int gdg) {
+  extern __shared__ PlanI8 plans[];
+  __shared__ unsigned red[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int slot = warp / wpp, part = warp - slot * wpp, slots = 8 / wpp;
+  const long long item = (long long)blockIdx.x * slots + slot;
+  const bool live = item < (long long)np * g.G;
+  const int gi = live ? (int)(item / np) : 0, lp = live ? (int)(item - (long long)gi * np) : 0;
+  const long long pix = p0 + lp;
+  const int n = (int)(pix / g.P), p = (int)(pix - (long long)n * g.P);
+  const int oy = p / g.Wo, ox = p - oy * g.Wo;
+  const int dg0 = gi * g.Cg / g.cpg;  // the group's first deformable group; gdg of them
+  PlanI8* mine = plans + slot * g.kk * gdg;
+  if (live) {
+    for (int i = part * 32 + lane; i < g.kk * gdg; i += wpp * 32) {
+      const int k = i / gdg, dgi = dg0 + i - k * gdg;
+      const int ki = k / g.kw, kj = k - ki * g.kw;
+      const long long oi = off_h_index(g, n, dgi, k, p);
+      float h, w;
+      sample_pos(g, oy, ox, ki, kj, ld<T>(off, oi), ld<T>(off, oi + g.P), h, w);
+      float m = 1.f;
+      if (g.use_mask) {
+        m = ld<T>(mask, mask_index(g, n, dgi, k, p));
+        if (g.mask_logits) m = 1.f / (1.f + expf(-m));
+      }
+      const Sample sp = make_sample(h, w, g.H, g.W);
+      PlanI8 q;
+      // a dropped corner: offset -1, not read
+      q.at[0] = sp.live & 1u ? sp.i1 * g.C : -1;
+      q.at[1] = sp.live & 2u ? sp.i2 * g.C : -1;
+      q.at[2] = sp.live & 4u ? sp.i3 * g.C : -1;
+      q.at[3] = sp.live & 8u ? sp.i4 * g.C : -1;
+      q.w[0] = sp.w1 * m;
+      q.w[1] = sp.w2 * m;
+      q.w[2] = sp.w3 * m;
+      q.w[3] = sp.w4 * m;
+      mine[i] = q;
+    }
+  }
+  __syncthreads();
+  const int cvec = g.Cg / 8, nvec = live ? g.kk * cvec : 0;
+  const long long img = (long long)n * g.HW * g.C;
+  float v[NV][8];
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    const int idx = part * 32 + lane + i * 32 * wpp;
+    if (idx < nvec) {
+      const int k = idx / cvec, ch = gi * g.Cg + (idx - k * cvec) * 8;
+      const PlanI8 q = mine[k * gdg + ch / g.cpg - dg0];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (q.at[c] >= 0) {
+          float u[8];
+          ld8<T>(x, img + q.at[c] + ch, u);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[i][j] += q.w[c] * u[j];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[i][j]));
+    }
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (wpp > 1) {  // the item's warps agree on its largest value
+    if (lane == 0) red[warp] = top;
+    __syncthreads();
+    for (int w = 0; w < wpp; ++w) top = max(top, red[slot * wpp + w]);
+  }
+  if (!live) return;
+  const float s = scale_of(top);
+  const bool ok = usable_scale(s);
+  signed char* out = col + ((long long)gi * np + lp) * kp;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int idx = part * 32 + lane + i * 32 * wpp;
+    if (idx < nvec) *reinterpret_cast<uint2*>(out + 8 * idx) = codes8(v[i], s, ok);
+  }
+  if (part == 0 && lane == 0) scale[(long long)gi * np + lp] = s;
+}
+
+template <int T, int NV>
+cudaError_t sample8_form(const Geom& g, const void* x, const void* off, const void* mask,
+                         long long p0, int np, signed char* col, int kp, float* scale, int wpp,
+                         int gdg, cudaStream_t stream) {
+  const long long items = (long long)np * g.G;
+  const int slots = 8 / wpp;
+  const size_t smem = sizeof(PlanI8) * g.kk * gdg * slots;
+  auto kern = sample8_i8_kernel<T, NV>;
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), (int)smem);
+  if (e != cudaSuccess) return e;
+  kern<<<(unsigned)((items + slots - 1) / slots), 256, smem, stream>>>(
+      g, x, off, mask, p0, np, col, kp, scale, wpp, gdg);
+  return cudaGetLastError();
+}
+
+// Products of up to NT tokens: a token does not fill a tensor-core tile, and
+// the weight is read once whatever the tokens are, so this is a matter of
+// reading it at full width.  A block codes the tokens for itself (they lie in
+// L2; a launch of its own would cost as much as the whole product), keeps the
+// codes in shared memory and gives each warp ROWS rows of the weight: lane l
+// multiplies 16-byte vectors l, l + 32, ... with the four-way integer dot
+// product.  The first vectors are on their way while the tokens are coded.
+constexpr int kFewAhead = 8;  // 16-byte weight vectors a lane has on its way
+
+template <int T, int NT, int ROWS>
+__global__ void __launch_bounds__(256)
+few_tokens_kernel(const void* __restrict__ x, const float* __restrict__ x_scale, int tokens,
+                  int K, int N, const signed char* __restrict__ w,
+                  const float* __restrict__ w_scale, const void* __restrict__ bias, int bias_type,
+                  void* __restrict__ out, int out_type) {
+  extern __shared__ uint4 xq[];  // [NT][K / 16]
+  __shared__ unsigned red[NT][8];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int vecs = K / 16;
+  const int row0 = (blockIdx.x * 8 + warp) * ROWS;
+  constexpr int AHEAD = kFewAhead / ROWS;
+  uint4 wv[ROWS][AHEAD];
+  const uint4* wr[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    wr[r] = reinterpret_cast<const uint4*>(w + (long long)min(row0 + r, N - 1) * K);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (lane + 32 * u < vecs) wv[r][u] = __ldg(wr[r] + lane + 32 * u);
+  }
+  float scale[NT];
+  if constexpr (T == 3) {
+    const uint4* xv = static_cast<const uint4*>(x);
+    for (int i = tid; i < NT * vecs; i += 256)
+      xq[i] = i < tokens * vecs ? __ldg(xv + i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) scale[t] = t < tokens ? __ldg(x_scale + t) : 0.f;
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      unsigned top = 0;
+      if (t < tokens)
+        for (int c = tid; c < K / 8; c += 256) {
+          float v[8];
+          ld8<T>(x, (long long)t * K + 8LL * c, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[j]));
+        }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) red[t][warp] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      unsigned top = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, red[t][i]);
+      const float s = scale_of(top);
+      const bool ok = usable_scale(s);
+      scale[t] = s;
+      uint2* dst = reinterpret_cast<uint2*>(xq + (long long)t * vecs);
+      for (int c = tid; c < K / 8; c += 256) {
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (t < tokens) ld8<T>(x, (long long)t * K + 8LL * c, v);
+        dst[c] = codes8(v, s, ok);
+      }
+    }
+    __syncthreads();
+  }
+  if (row0 >= N) return;
+  int acc[ROWS][NT];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[r][t] = 0;
+  for (int c0 = 0; c0 < vecs; c0 += 32 * AHEAD) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int c = c0 + 32 * u + lane;
+      if (c < vecs) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const uint4 xv = xq[t * vecs + c];
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) {
+            acc[r][t] = __dp4a((int)wv[r][u].x, (int)xv.x, acc[r][t]);
+            acc[r][t] = __dp4a((int)wv[r][u].y, (int)xv.y, acc[r][t]);
+            acc[r][t] = __dp4a((int)wv[r][u].z, (int)xv.z, acc[r][t]);
+            acc[r][t] = __dp4a((int)wv[r][u].w, (int)xv.w, acc[r][t]);
+          }
+        }
+        const int next = c + 32 * AHEAD;
+        if (next < vecs) {
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) wv[r][u] = __ldg(wr[r] + next);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int row = row0 + r;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int sum = __reduce_add_sync(0xffffffffu, acc[r][t]);
+      if (lane == t && t < tokens && row < N) {
+        float y = (float)sum * scale[t] * __ldg(w_scale + row);
+        if (bias != nullptr)
+          y += bias_type == kF32 ? ld<kF32>(bias, row)
+               : bias_type == kBF16T ? ld<kBF16T>(bias, row) : ld<kF16T>(bias, row);
+        const long long at = (long long)t * N + row;
+        if (out_type == kF32) static_cast<float*>(out)[at] = y;
+        else if (out_type == kBF16T) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(y);
+        else static_cast<__half*>(out)[at] = __float2half_rn(y);
+      }
+    }
+  }
+}
+
+template <int T, int NT, int ROWS>
+cudaError_t few_form(const void* x, const float* x_scale, int tokens, int K, int N,
+                     const signed char* w, const float* w_scale, const void* bias, int bias_type,
+                     void* out, int out_type, cudaStream_t stream) {
+  auto kern = few_tokens_kernel<T, NT, ROWS>;
+  const int smem = NT * K;
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
+  if (e != cudaSuccess) return e;
+  kern<<<(N + 8 * ROWS - 1) / (8 * ROWS), 256, smem, stream>>>(
+      x, x_scale, tokens, K, N, w, w_scale, bias, bias_type, out, out_type);
+  return cudaGetLastError();
+}
+
+template <int T>
+cudaError_t few_type(const void* x, const float* x_scale, int tokens, int K, int N,
+                     const signed char* w, const float* w_scale, const void* bias, int bias_type,
+                     void* out, int out_type, cudaStream_t stream) {
+  auto form = tokens <= 1 ? few_form<T, 1, 1> : tokens <= 2 ? few_form<T, 2, 1>
+              : tokens <= 4 ? few_form<T, 4, 2> : few_form<T, 8, 2>;
+  return form(x, x_scale, tokens, K, N, w, w_scale, bias, bias_type, out, out_type, stream);
+}
+
 template <int T>
 cudaError_t sample_type(const Geom& g, const void* x, const void* off, const void* mask,
                         long long p0, int np, signed char* col, int kp, float* scale,
                         cudaStream_t stream) {
   const long long items = (long long)np * g.G;
+  // eights of channels within each group and deformable group, plans and
+  // registers that hold an item: the vector kernel
+  const int gdg = g.Cg >= g.cpg ? g.Cg / g.cpg : 1;
+  const bool nested = g.Cg % g.cpg == 0 || g.cpg % g.Cg == 0;
+  const long long nvec = (long long)g.kk * g.Cg / 8;
+  if (g.Cg % 8 == 0 && g.cpg % 8 == 0 && nested && nvec <= 9 * 32 * 8 &&
+      (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
+      sizeof(PlanI8) * g.kk * gdg * 8 <= 96 * 1024) {
+    int wpp = 1;
+    while (nvec > 9LL * 32 * wpp) wpp *= 2;
+    const long long nv = (nvec + 32 * wpp - 1) / (32 * wpp);
+    auto form = nv <= 1 ? sample8_form<T, 1> : nv <= 3 ? sample8_form<T, 3>
+                : nv <= 5 ? sample8_form<T, 5> : sample8_form<T, 9>;
+    return form(g, x, off, mask, p0, np, col, kp, scale, wpp, gdg, stream);
+  }
   const size_t one = (size_t)g.kk * g.Cg * sizeof(float);
   if (one <= 200 * 1024) {
     int warps = 8;
@@ -164,11 +517,35 @@ cudaError_t launch_quantize_rows(const void* x, int type, long long rows, int co
                                  cudaStream_t stream) {
   if (rows <= 0) return cudaSuccess;
   if (rows > (1LL << 31) - 1) return cudaErrorInvalidValue;
+  const int es = type == kF32 ? 4 : 2;
+  if (cols % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ldx * es % 16 == 0 &&
+      (reinterpret_cast<uintptr_t>(q) & 7) == 0 && ldq % 8 == 0) {
+    auto kern8 = type == kF32 ? quantize_rows8_kernel<kF32>
+                 : type == kBF16T ? quantize_rows8_kernel<kBF16T>
+                                  : quantize_rows8_kernel<kF16T>;
+    const int vecs = cols / 8, warps = (vecs + 31) / 32;
+    kern8<<<(unsigned)rows, 32 * (warps < 8 ? warps : 8), 0, stream>>>(x, vecs, ldx, q, ldq,
+                                                                       scale);
+    return cudaGetLastError();
+  }
   auto kern = type == kF32 ? quantize_rows_kernel<kF32>
               : type == kBF16T ? quantize_rows_kernel<kBF16T>
                                : quantize_rows_kernel<kF16T>;
   kern<<<(unsigned)rows, 256, 0, stream>>>(x, cols, ldx, q, ldq, scale);
   return cudaGetLastError();
+}
+
+bool few_tokens_fit(int64_t tokens, int64_t K) {
+  const int64_t nt = tokens <= 1 ? 1 : tokens <= 2 ? 2 : tokens <= 4 ? 4 : 8;
+  return tokens <= 8 && K % 16 == 0 && nt * K <= 96 * 1024;
+}
+
+cudaError_t launch_few_tokens(const void* x, int x_type, const float* x_scale, int tokens, int K,
+                              int N, const signed char* w, const float* w_scale, const void* bias,
+                              int bias_type, void* out, int out_type, cudaStream_t stream) {
+  auto run = x_type == kF32 ? few_type<kF32> : x_type == kBF16T ? few_type<kBF16T>
+             : x_type == kF16T ? few_type<kF16T> : few_type<3>;
+  return run(x, x_scale, tokens, K, N, w, w_scale, bias, bias_type, out, out_type, stream);
 }
 
 cudaError_t launch_repack_i8(const signed char* in, long long rows, int cols, signed char* out,

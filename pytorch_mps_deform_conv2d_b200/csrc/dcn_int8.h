@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cuda_runtime.h>
+#include <stdint.h>
 
 #include "dcn_common.cuh"
 #include "dcn_gemm.h"
@@ -16,6 +17,13 @@ namespace dcn {
 cudaError_t launch_quantize_rows(const void* x, int type, long long rows, int cols, long long ldx,
                                  signed char* q, long long ldq, float* scale,
                                  cudaStream_t stream);
+// Whether a product of so few tokens runs as one kernel that codes the tokens
+// itself, and that kernel: x (tokens, K) of `x_type` (3: int8 with x_scale),
+// weight (N, K), both dense and 16-byte aligned.
+bool few_tokens_fit(int64_t tokens, int64_t K);
+cudaError_t launch_few_tokens(const void* x, int x_type, const float* x_scale, int tokens, int K,
+                              int N, const signed char* w, const float* w_scale, const void* bias,
+                              int bias_type, void* out, int out_type, cudaStream_t stream);
 // 8-bit rows into rows of pitch `ldo`.
 cudaError_t launch_repack_i8(const signed char* in, long long rows, int cols, signed char* out,
                              long long ldo, cudaStream_t stream);
