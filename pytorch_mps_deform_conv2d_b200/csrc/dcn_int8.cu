@@ -216,6 +216,61 @@ sample_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ of
   if (lane == 0) scale[(long long)gi * np + lp] = s;
 }
 
+// Two fp32 values side by side, and a multiply-add of both at once.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float max_abs_nan(float top, float v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(v)));
+  return r;
+}
+// Eight values as they lie in memory (zeros when not wanted), and the j-th pair
+// of them as fp32.
+template <int T>
+struct Raw8 {
+  uint4 w[T == kF32 ? 2 : 1];
+};
+template <int T>
+__device__ __forceinline__ Raw8<T> ld8_if(const void* p, long long i, bool want) {
+  Raw8<T> r;
+  constexpr int N = T == kF32 ? 2 : 1;
+  const uint4* q = reinterpret_cast<const uint4*>(static_cast<const char*>(p) +
+                                                  i * (T == kF32 ? 4 : 2));
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    r.w[k] = make_uint4(0, 0, 0, 0);
+    if (want) r.w[k] = __ldg(q + k);
+  }
+  return r;
+}
+template <int T>
+__device__ __forceinline__ uint64_t raw_pair(const Raw8<T>& r, int j) {
+  if constexpr (T == kF32) {
+    const uint4 u = r.w[j >> 1];
+    return j & 1 ? pair(__uint_as_float(u.z), __uint_as_float(u.w))
+                 : pair(__uint_as_float(u.x), __uint_as_float(u.y));
+  } else {
+    const uint32_t w = j == 0 ? r.w[0].x : j == 1 ? r.w[0].y : j == 2 ? r.w[0].z : r.w[0].w;
+    if constexpr (T == kBF16T)
+      return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return pair(f.x, f.y);
+  }
+}
+
 // Channels in eights (per group, per deformable group).  WPP warps share an
 // item, so that each lane holds at most NV vectors of eight samples in
 // registers from the gather to their codes: the input is gathered once and
@@ -275,43 +330,64 @@ sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ o
   __syncthreads();
   const int cvec = g.Cg / 8, nvec = live ? g.kk * cvec : 0;
   const long long img = (long long)n * g.HW * g.C;
-  float v[NV][8];
-  unsigned top = 0;
+  uint64_t v[NV][4];  // pairs of fp32
+  float top = 0.f;    // NaN stays
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    for (int j = 0; j < 4; ++j) v[i][j] = 0;
     const int idx = part * 32 + lane + i * 32 * wpp;
     if (idx < nvec) {
       const int k = idx / cvec, ch = gi * g.Cg + (idx - k * cvec) * 8;
-      const PlanI8 q = mine[k * gdg + ch / g.cpg - dg0];
+      const PlanI8 q = mine[k * gdg + (gdg > 1 ? ch / g.cpg - dg0 : 0)];
+      Raw8<T> raw[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) raw[c] = ld8_if<T>(x, img + q.at[c] + ch, q.at[c] >= 0);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        if (q.at[c] >= 0) {
-          float u[8];
-          ld8<T>(x, img + q.at[c] + ch, u);
+        const uint64_t w2 = pair(q.w[c], q.w[c]);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] += q.w[c] * u[j];
-        }
+        for (int j = 0; j < 4; ++j) v[i][j] = fma2(raw_pair<T>(raw[c], j), w2, v[i][j]);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[i][j]));
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = unpair(v[i][j]);
+        top = max_abs_nan(max_abs_nan(top, f.x), f.y);
+      }
     }
   }
-  top = __reduce_max_sync(0xffffffffu, top);
+  unsigned bits = __reduce_max_sync(0xffffffffu, abs_bits(top));
   if (wpp > 1) {  // the item's warps agree on its largest value
-    if (lane == 0) red[warp] = top;
+    if (lane == 0) red[warp] = bits;
     __syncthreads();
-    for (int w = 0; w < wpp; ++w) top = max(top, red[slot * wpp + w]);
+    for (int w = 0; w < wpp; ++w) bits = max(bits, red[slot * wpp + w]);
   }
   if (!live) return;
-  const float s = scale_of(top);
+  const float s = scale_of(bits);
   const bool ok = usable_scale(s);
+  // one reciprocal for the item: the samples are rounded sums already, so the
+  // codes are within those roundings of the formula's
+  const float inv = ok ? 1.f / s : 0.f;
   signed char* out = col + ((long long)gi * np + lp) * kp;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int idx = part * 32 + lane + i * 32 * wpp;
-    if (idx < nvec) *reinterpret_cast<uint2*>(out + 8 * idx) = codes8(v[i], s, ok);
+    if (idx < nvec) {
+      // v inv + 1.5 * 2^23: rounded to the nearest whole number, its low byte
+      // the code (|v inv| is 127 at most, up to a rounding)
+      uint32_t b[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = unpair(v[i][j]);
+        b[2 * j] = __float_as_uint(fmaf(f.x, inv, 12582912.f));
+        b[2 * j + 1] = __float_as_uint(fmaf(f.y, inv, 12582912.f));
+      }
+      uint2 c;
+      c.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+      c.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
+      if (!ok) c = make_uint2(0, 0);
+      *reinterpret_cast<uint2*>(out + 8 * idx) = c;
+    }
   }
   if (part == 0 && lane == 0) scale[(long long)gi * np + lp] = s;
 }
