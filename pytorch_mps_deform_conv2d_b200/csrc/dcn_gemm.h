@@ -27,7 +27,7 @@ struct GemmOperand {
 
 enum GemmEpilogue {
   // v = acc * scale[b] * factor, stored as fp16 terms (`out16`); with `sym`
-  // only tiles that reach the upper triangle are computed, and mirrored
+  // large products compute the upper triangle of tiles and mirror it
   kEpiTerms = 0,
   // the same of v = (diag on the diagonal) + lin * L + acc * factor, L the
   // two-term matrix `lin16` of the same layout
@@ -76,6 +76,9 @@ struct GemmProblem {
   int M, N, K, batch;
   int a_batch_mod;  // batch index of A is b % a_batch_mod (0: b)
   bool int8, sym;
+  bool fine;        // two-term operands: sums to fp32's accuracy
+  bool after_ours;  // the launch before is one of this library's products, or
+                    // another kernel whose writes this one may wait for late
   GemmEpiArgs epi;
   long long wait_limit;
   int no_async;

@@ -277,6 +277,8 @@ cudaError_t launch_ortho(const OrthoShape& s, const OrthoChunk& c, void* workspa
     g.K = K;
     g.batch = c.count;
     g.sym = sym;
+    g.fine = s.type == kF32;
+    g.after_ours = true;
     g.epi = epi;
     g.wait_limit = wait_limit;
     g.no_async = no_async;
