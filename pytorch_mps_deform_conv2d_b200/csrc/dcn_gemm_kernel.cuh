@@ -162,6 +162,24 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t addr, uint32_t cols) {
     tc::tmem_dealloc(addr, cols);
 }
 
+// One lane of a converged warp.  The instructions below take their operands
+// from uniform registers; under `lane == 0` the compiler does not know that one
+// thread runs and wraps each in a loop over the active ones: 800 cycles a K
+// slice, measured, against 512 of its products.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "elect.sync _|p, 0xFFFFFFFF;\n"
+      "selp.b32 %0, 1, 0, p;\n}\n"
+      : "=r"(r));
+  return r != 0;
+}
+// A wait of the whole warp: all of its lanes come to the same answer.
+__device__ __forceinline__ bool wait_warp(const tc::Watch& w, uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, tc::wait(w, bar, parity));
+}
+
 // ---- clusters ----
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -546,7 +564,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
 
   if (warp == 0) {
     // ------------------------------ loads ------------------------------
-    if (lane == 0 && !g.no_async) {
+    if (elect_one() && !g.no_async) {
       int it = 0;
       bool ok = true;
       for (int t = first_tile; t < g.tiles && ok; t += tile_step) {
@@ -594,71 +612,73 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------ products ------------------------------
-    if (lane == 0 && (!PAIR || rank == 0)) {
+    if (!PAIR || rank == 0) {
       constexpr uint32_t id = idesc<I8, AT, BT>(F::TM, BN);
       const uint32_t cross = tmem + (uint32_t)(F::BUFS * BN);
+      // 16 K values (32 of int8): 32 bytes along a row, or 16 rows of 128
+      constexpr uint64_t ka = AT ? 2048 >> 4 : 32 >> 4, kb = BT ? 2048 >> 4 : 32 >> 4;
+      constexpr uint64_t la = F::A_TERM >> 4, lb = F::B_TERM >> 4;
+      constexpr int RUN = UNIT == 2 ? 2 : 4;  // steps of 16 issued at once
       int it = 0, n = 0, unit = 0;
       bool ok = true;
       for (int t = first_tile; t < g.tiles && ok; t += tile_step, ++n) {
         uint32_t d = 0;
         int steps = 0;  // of 16 values of K in the current unit
-        for (int k = 0; k < ksteps && ok; ++k, ++it) {
+        for (int k = 0; k < ksteps; ++k, ++it) {
           const int st = it % STAGES;
-          if (!tc::wait(watch, &full[st], (it / STAGES) & 1)) {
-            ok = false;
-            break;
-          }
+          ok = wait_warp(watch, &full[st], (it / STAGES) & 1);
+          if (F::CROSS && ok && k == 0 && n > 0)
+            ok = wait_warp(watch, cross_empty, (n - 1) & 1);
+          if (!ok) break;
           tc::tc_fence_after();
           const uint32_t sa = s0 + st * F::STAGE, sb = sa + TA * F::A_TERM;
           const uint64_t da = AT ? sdesc_k_rows(sa) : tc::sdesc_sw128(sa);
           const uint64_t db = BT ? sdesc_k_rows(sb) : tc::sdesc_sw128(sb);
-          // 16 K values (32 of int8): 32 bytes along a row, or 16 rows of 128
-          constexpr uint64_t ka = AT ? 2048 >> 4 : 32 >> 4, kb = BT ? 2048 >> 4 : 32 >> 4;
-          constexpr uint64_t la = F::A_TERM >> 4, lb = F::B_TERM >> 4;
-          if constexpr (F::CROSS) {
-            if (k == 0 && n > 0 && !tc::wait(watch, cross_empty, (n - 1) & 1)) {
-              ok = false;
-              break;
-            }
-          }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (F::CROSS) {
-              if (j % 2 == 0) {  // a unit's cross terms before its accumulator is needed
+          for (int j = 0; j < 4; j += RUN) {
+            if constexpr (F::CROSS) {  // a unit's cross terms before its accumulator is needed
+              if (elect_one()) {
 #pragma unroll
-                for (int i = j; i < j + 2; ++i) {
+                for (int i = j; i < j + RUN; ++i) {
                   umma<I8, PAIR>(cross, da + i * ka, db + lb + i * kb, id, (k | i) != 0 ? 1u : 0u);
                   umma<I8, PAIR>(cross, da + la + i * ka, db + i * kb, id, 1u);
                 }
               }
+              __syncwarp();
             }
             if (steps == 0) {
               const int buf = unit % F::BUFS, use = unit / F::BUFS;
-              if (use > 0 && !tc::wait(watch, &acc_empty[buf], (use - 1) & 1)) {
-                ok = false;
-                break;
-              }
+              if (use > 0) ok = wait_warp(watch, &acc_empty[buf], (use - 1) & 1);
+              if (!ok) break;
               tc::tc_fence_after();
               d = tmem + (uint32_t)(buf * BN);
             }
-            umma<I8, PAIR>(d, da + j * ka, db + j * kb, id, steps != 0 ? 1u : 0u);
-            if constexpr (!F::CROSS && TB == 2)
-              umma<I8, PAIR>(d, da + j * ka, db + lb + j * kb, id, 1u);
-            if constexpr (!F::CROSS && TA == 2)
-              umma<I8, PAIR>(d, da + la + j * ka, db + j * kb, id, 1u);
-            ++steps;
-            if (steps == UNIT || (k + 1 == ksteps && j == 3)) {
-              commit<PAIR>(&acc_full[unit % F::BUFS]);
+            const bool last = j + RUN == 4;
+            const bool unit_done = steps + RUN == UNIT || (last && k + 1 == ksteps);
+            if (elect_one()) {
+#pragma unroll
+              for (int i = j; i < j + RUN; ++i) {
+                umma<I8, PAIR>(d, da + i * ka, db + i * kb, id, steps + i - j != 0 ? 1u : 0u);
+                if constexpr (!F::CROSS && TB == 2)
+                  umma<I8, PAIR>(d, da + i * ka, db + lb + i * kb, id, 1u);
+                if constexpr (!F::CROSS && TA == 2)
+                  umma<I8, PAIR>(d, da + la + i * ka, db + i * kb, id, 1u);
+              }
+              if (unit_done) commit<PAIR>(&acc_full[unit % F::BUFS]);
+              if (last) commit<PAIR>(&empty[st]);
+              if (F::CROSS && last && k + 1 == ksteps) commit<PAIR>(cross_full);
+            }
+            __syncwarp();
+            steps += RUN;
+            if (unit_done) {
               ++unit;
               steps = 0;
             }
           }
-          if (ok) commit<PAIR>(&empty[st]);
+          if (!ok) break;
         }
-        if constexpr (F::CROSS)
-          if (ok) commit<PAIR>(cross_full);
       }
-      if (tc::aborted(watch)) {  // every product issued so far completes before the CTA leaves
+      if (!ok && elect_one()) {  // every product issued so far completes before the CTA leaves
         commit<PAIR>(drain);
         tc::drain_wait(drain, 0, g.wait_limit);
       }
