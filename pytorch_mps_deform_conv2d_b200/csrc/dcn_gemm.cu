@@ -1,6 +1,7 @@
 // dcn_gemm.cu -- int8 products, and the choice of the form (see
 // dcn_gemm_kernel.cuh).
 #include "dcn_gemm_kernel.cuh"
+#include "dcn_ortho_chain.h"
 
 namespace dcn {
 
@@ -17,11 +18,12 @@ cudaError_t launch_gemm(const GemmProblem& p, cudaStream_t stream) {
 }
 
 cudaError_t read_gemm_status(int* status, bool clear, cudaStream_t stream) {
-  int v[3] = {0, 0, 0};
+  int v[4] = {0, 0, 0, 0};
   cudaError_t e = read_status(&v[0], clear, stream);
   if (e == cudaSuccess) e = read_gemm_f16_status(&v[1], clear, stream);
   if (e == cudaSuccess) e = read_gemm_f16x2_status(&v[2], clear, stream);
-  *status = v[0] | v[1] | v[2];
+  if (e == cudaSuccess) e = read_chain_status(&v[3], clear, stream);
+  *status = v[0] | v[1] | v[2] | v[3];
   return e;
 }
 

@@ -26,16 +26,13 @@
 // K = 4096 470; the steps of an orthogonalisation multiply that by about 100.
 // So an accumulator only ever holds a short run of K (a unit), and the epilogue
 // warps add the units in registers, rounding to nearest.  For fp32 results
-// units of 32 values, the cross terms (2^-11 as large) in an accumulator of
-// their own; what 32 lose on average, 1.1 units of 2^-24 (0.8 for terms of both
-// signs, 1.4 for squares), is added back.  For 16-bit results units of 256.
+// units of 32 values, the cross terms (2^-11 as large, and so are their losses)
+// before hi hi; what is lost on average, 1.1 units of 2^-24 (0.8 for terms of
+// both signs, 1.4 for squares), is added back.  For 16-bit results units of 256.
 #pragma once
 
+#include "dcn_dense_common.cuh"
 #include "dcn_gemm.h"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include "dcn_launch.h"
 #include "dcn_tc_common.cuh"
 #include "dcn_tma.h"
@@ -43,6 +40,8 @@
 namespace dcn {
 
 namespace {
+
+using namespace dense;
 
 __device__ int g_gemm_status = 0;
 
@@ -53,8 +52,6 @@ constexpr int kSmemMax = 227 * 1024;
 constexpr int kStageWarp = 32 * 17 * 4;  // a warp's transposition buffer
 // alignment, barriers, channel scales, transposition
 constexpr int kMiscBytes = 1024 + 256 + 2048 + EPI_WARPS * kStageWarp;
-// 1.1 units of 2^-24 (see the top of the file)
-constexpr float kUnitLoss = 6.5565e-8f;
 
 struct GemmArgs {
   int M, N, K;
@@ -81,35 +78,13 @@ struct Form {
   static constexpr int STAGES = FIT > 8 ? 8 : FIT;
   static constexpr int SMEM = STAGES * STAGE + kMiscBytes;
   static_assert(STAGES >= 3, "three stages at least");
-  static_assert((2 * STAGES + 10) * 8 <= 256, "room for the barriers");
-  // units small enough to need it keep the cross terms apart
-  static constexpr bool CROSS = TA == 2 && TB == 2 && UNIT == 2;
-  static constexpr int BUFS = CROSS ? (BN == 256 ? 1 : 3) : 2;
-  static constexpr int TMEM = (BUFS + (CROSS ? 1 : 0)) * BN;
-  static_assert((TMEM & (TMEM - 1)) == 0 && TMEM <= 512, "a power of two of columns");
+  static constexpr int BUFS = BN == 256 || UNIT == 0 ? 2 : 4;  // accumulators
+  static constexpr int TMEM = BUFS * BN;
+  static_assert((2 * STAGES + 2 * BUFS + 2) * 8 <= 256, "room for the barriers");
   static constexpr int COLS = BN / 2;  // of an epilogue warp
   static constexpr int PART_PITCH = BN + 4;  // floats a row of a partial sum
   static_assert(BN != 64 || STAGES * STAGE >= BM * PART_PITCH * 4, "room for a partial sum");
 };
-
-// 4-D tiled TMA load (no multicast): box at (x, y, term, matrix).  PAIR: the
-// barrier may be the other CTA's.
-template <bool PAIR>
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y,
-                                            int z, int w, uint32_t bar) {
-  if constexpr (PAIR)
-    asm volatile(
-        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
-        "bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
-        : "memory");
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
-        : "memory");
-}
 
 template <bool I8, bool PAIR>
 __device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
@@ -162,24 +137,6 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t addr, uint32_t cols) {
     tc::tmem_dealloc(addr, cols);
 }
 
-// One lane of a converged warp.  The instructions below take their operands
-// from uniform registers; under `lane == 0` the compiler does not know that one
-// thread runs and wraps each in a loop over the active ones: 800 cycles a K
-// slice, measured, against 512 of its products.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t r;
-  asm volatile(
-      "{\n.reg .pred p;\n"
-      "elect.sync _|p, 0xFFFFFFFF;\n"
-      "selp.b32 %0, 1, 0, p;\n}\n"
-      : "=r"(r));
-  return r != 0;
-}
-// A wait of the whole warp: all of its lanes come to the same answer.
-__device__ __forceinline__ bool wait_warp(const tc::Watch& w, uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, tc::wait(w, bar, parity));
-}
-
 // ---- clusters ----
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -208,15 +165,6 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
                : "memory");
   return v;
 }
-// ---- programmatic dependent launch: the prologue of a product runs beside the
-// end of the launch before it ----
-__device__ __forceinline__ void grid_wait() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-__device__ __forceinline__ void grid_launch_dependents() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
 // Instruction descriptors: fp16 x fp16 -> fp32 (bits 15 / 16: the operand's
 // rows run along K), and signed 8-bit -> int32.
 template <bool I8, bool AT, bool BT>
@@ -231,21 +179,6 @@ __device__ constexpr uint32_t idesc(int M, int N) {
 __device__ __forceinline__ uint64_t sdesc_k_rows(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(8192 >> 4) << 16) | (64ull << 32) |
          (1ull << 46) | (2ull << 61);
-}
-
-// 32 lanes x 32-bit, 32 consecutive columns.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-      "%30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
 }
 
 struct Tile {
@@ -289,51 +222,41 @@ __device__ __forceinline__ void store_f(void* p, long long i, float v) {
   else if constexpr (T == kBF16T) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
-template <int T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (T == kBF16T) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-template <int T>
-__device__ __forceinline__ float2 unpack2(uint32_t w) {
-  if constexpr (T == kBF16T)
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-
 // ---- epilogues: eight consecutive columns n .. n + 7 of row m < M ----
 
 // fp16 terms.  The pitch is a multiple of eight, so a chunk that starts inside
-// the row fits.  hi / lo return what was stored.
-__device__ __forceinline__ void terms8(const GemmArgs& g, float (&v)[8], int b, int m, int n,
+// the row fits.  lh, ll: the terms of the linear part (kEpiPoly); hi / lo return
+// what was stored.
+__device__ __forceinline__ uint4 linear8(const GemmArgs& g, int term, int b, int m, int n) {
+  const GemmEpiArgs& e = g.e;
+  if (e.mode != kEpiPoly || m >= g.M || n >= g.N) return make_uint4(0, 0, 0, 0);
+  return *reinterpret_cast<const uint4*>(e.lin16 + term * e.term_stride +
+                                         (long long)b * e.batch_stride +
+                                         (long long)m * e.pitch + n);
+}
+__device__ __forceinline__ void terms8(const GemmArgs& g, const float (&v)[8], int b, int m,
+                                       int n, const uint4& lh, const uint4& ll,
                                        uint32_t (&hi)[4], uint32_t (&lo)[4]) {
   const GemmEpiArgs& e = g.e;
   const long long at = (long long)b * e.batch_stride + (long long)m * e.pitch + n;
+  uint64_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = pair(v[2 * j], v[2 * j + 1]);
   if (e.mode == kEpiPoly) {
-    const uint4 h = *reinterpret_cast<const uint4*>(e.lin16 + at);
-    const uint4 l = *reinterpret_cast<const uint4*>(e.lin16 + e.term_stride + at);
-    const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 a = unpack2<kF16T>(hw[j]), c = unpack2<kF16T>(lw[j]);
-      v[2 * j] += e.lin * (a.x + c.x);
-      v[2 * j + 1] += e.lin * (a.y + c.y);
-    }
+    const uint64_t lin = pair(e.lin, e.lin);
+    w[0] = fma2(join2(lh.x, ll.x), lin, w[0]);
+    w[1] = fma2(join2(lh.y, ll.y), lin, w[1]);
+    w[2] = fma2(join2(lh.z, ll.z), lin, w[2]);
+    w[3] = fma2(join2(lh.w, ll.w), lin, w[3]);
     const int d = m - n;
+    if (d >= 0 && d < 8) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] += j == d ? e.diag : 0.f;
+      for (int j = 0; j < 4; ++j)
+        w[j] = add2(w[j], pair(d == 2 * j ? e.diag : 0.f, d == 2 * j + 1 ? e.diag : 0.f));
+    }
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    hi[j] = pack2<kF16T>(v[2 * j], v[2 * j + 1]);
-    const float2 h = unpack2<kF16T>(hi[j]);
-    lo[j] = pack2<kF16T>(v[2 * j] - h.x, v[2 * j + 1] - h.y);
-  }
+  for (int j = 0; j < 4; ++j) split2(w[j], hi[j], lo[j]);
   *reinterpret_cast<uint4*>(e.out16 + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
   if (e.out_terms == 2)
     *reinterpret_cast<uint4*>(e.out16 + e.term_stride + at) =
@@ -409,6 +332,12 @@ __device__ __forceinline__ void terms32(const GemmArgs& g, float (&v)[32], const
                                         int n0) {
   const GemmEpiArgs& e = g.e;
   if (m >= g.M) return;
+  uint4 lh[4], ll[4];  // on their way together
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    lh[c] = linear8(g, 0, T.b, m, n0 + 8 * c);
+    ll[c] = linear8(g, 1, T.b, m, n0 + 8 * c);
+  }
 #pragma unroll
   for (int c = 0; c < 32; c += 8) {
     const int n = n0 + c;
@@ -417,7 +346,7 @@ __device__ __forceinline__ void terms32(const GemmArgs& g, float (&v)[32], const
 #pragma unroll
     for (int j = 0; j < 8; ++j) u[j] = v[c + j];
     uint32_t hi[4], lo[4];
-    terms8(g, u, T.b, m, n, hi, lo);
+    terms8(g, u, T.b, m, n, lh[c / 8], ll[c / 8], hi, lo);
     if (T.mirrored) {  // lanes hold neighbouring columns of the mirrored rows
       unsigned short* out =
           e.out16 + (long long)T.b * e.batch_stride + (long long)n * e.pitch + m;
@@ -519,9 +448,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + F::BUFS;
-  uint64_t* cross_full = acc_empty + F::BUFS;
-  uint64_t* cross_empty = cross_full + 1;
-  uint64_t* drain = cross_empty + 1;
+  uint64_t* drain = acc_empty + F::BUFS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   const tc::Watch watch{abort_flag, &g_gemm_status, kStatusDense, g.wait_limit};
@@ -545,8 +472,6 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
       tc::mbar_init(&acc_full[a], 1);
       tc::mbar_init(&acc_empty[a], EPI_WARPS * (PAIR ? 2 : 1));
     }
-    tc::mbar_init(cross_full, 1);
-    tc::mbar_init(cross_empty, EPI_WARPS * (PAIR ? 2 : 1));
     tc::mbar_init(drain, 1);
     *abort_flag = 0;
     tc::fence_mbar_init();
@@ -614,7 +539,6 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
     // ------------------------------ products ------------------------------
     if (!PAIR || rank == 0) {
       constexpr uint32_t id = idesc<I8, AT, BT>(F::TM, BN);
-      const uint32_t cross = tmem + (uint32_t)(F::BUFS * BN);
       // 16 K values (32 of int8): 32 bytes along a row, or 16 rows of 128
       constexpr uint64_t ka = AT ? 2048 >> 4 : 32 >> 4, kb = BT ? 2048 >> 4 : 32 >> 4;
       constexpr uint64_t la = F::A_TERM >> 4, lb = F::B_TERM >> 4;
@@ -627,8 +551,6 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
         for (int k = 0; k < ksteps; ++k, ++it) {
           const int st = it % STAGES;
           ok = wait_warp(watch, &full[st], (it / STAGES) & 1);
-          if (F::CROSS && ok && k == 0 && n > 0)
-            ok = wait_warp(watch, cross_empty, (n - 1) & 1);
           if (!ok) break;
           tc::tc_fence_after();
           const uint32_t sa = s0 + st * F::STAGE, sb = sa + TA * F::A_TERM;
@@ -636,16 +558,6 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
           const uint64_t db = BT ? sdesc_k_rows(sb) : tc::sdesc_sw128(sb);
 #pragma unroll
           for (int j = 0; j < 4; j += RUN) {
-            if constexpr (F::CROSS) {  // a unit's cross terms before its accumulator is needed
-              if (elect_one()) {
-#pragma unroll
-                for (int i = j; i < j + RUN; ++i) {
-                  umma<I8, PAIR>(cross, da + i * ka, db + lb + i * kb, id, (k | i) != 0 ? 1u : 0u);
-                  umma<I8, PAIR>(cross, da + la + i * ka, db + i * kb, id, 1u);
-                }
-              }
-              __syncwarp();
-            }
             if (steps == 0) {
               const int buf = unit % F::BUFS, use = unit / F::BUFS;
               if (use > 0) ok = wait_warp(watch, &acc_empty[buf], (use - 1) & 1);
@@ -656,17 +568,23 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
             const bool last = j + RUN == 4;
             const bool unit_done = steps + RUN == UNIT || (last && k + 1 == ksteps);
             if (elect_one()) {
+              if constexpr (TA + TB > 2) {  // the small terms first
 #pragma unroll
-              for (int i = j; i < j + RUN; ++i) {
-                umma<I8, PAIR>(d, da + i * ka, db + i * kb, id, steps + i - j != 0 ? 1u : 0u);
-                if constexpr (!F::CROSS && TB == 2)
-                  umma<I8, PAIR>(d, da + i * ka, db + lb + i * kb, id, 1u);
-                if constexpr (!F::CROSS && TA == 2)
-                  umma<I8, PAIR>(d, da + la + i * ka, db + i * kb, id, 1u);
+                for (int i = j; i < j + RUN; ++i) {
+                  if constexpr (TB == 2)
+                    umma<I8, PAIR>(d, da + i * ka, db + lb + i * kb, id,
+                                   steps + i - j != 0 ? 1u : 0u);
+                  if constexpr (TA == 2)
+                    umma<I8, PAIR>(d, da + la + i * ka, db + i * kb, id,
+                                   TB == 2 || steps + i - j != 0 ? 1u : 0u);
+                }
               }
+#pragma unroll
+              for (int i = j; i < j + RUN; ++i)
+                umma<I8, PAIR>(d, da + i * ka, db + i * kb, id,
+                               TA + TB > 2 || steps + i - j != 0 ? 1u : 0u);
               if (unit_done) commit<PAIR>(&acc_full[unit % F::BUFS]);
               if (last) commit<PAIR>(&empty[st]);
-              if (F::CROSS && last && k + 1 == ksteps) commit<PAIR>(cross_full);
             }
             __syncwarp();
             steps += RUN;
@@ -753,10 +671,11 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
         release(&acc_empty[buf]);
       } else {
         const float f = g.e.factor * (g.e.scale != nullptr ? __ldg(g.e.scale + T.b) : 1.f);
-        float acc[COLS];
+        uint64_t acc[COLS / 2];
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
+        for (int c = 0; c < COLS / 2; ++c) acc[c] = 0;
         bool ok = true;
+#pragma unroll 1
         for (int u = 0; u < units; ++u, ++unit) {
           const int buf = unit % F::BUFS;
           if (!tc::wait(watch, &acc_full[buf], (unit / F::BUFS) & 1)) {
@@ -770,31 +689,25 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
             tmem_ld32(lanes + (uint32_t)(buf * BN + c), r);
             tc::tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) acc[c + j] += __uint_as_float(r[j]);
+            for (int j = 0; j < 16; ++j)
+              acc[c / 2 + j] = add2(acc[c / 2 + j], pair(__uint_as_float(r[2 * j]),
+                                                         __uint_as_float(r[2 * j + 1])));
           }
           release(&acc_empty[buf]);
         }
         if (!ok) break;
-        if constexpr (F::CROSS) {
-          if (!tc::wait(watch, cross_full, n & 1)) break;
-          tc::tc_fence_after();
+        if constexpr (UNIT == 2) {
+          const uint64_t loss = pair(kUnitLoss, kUnitLoss);
 #pragma unroll
-          for (int c = 0; c < COLS; c += 32) {
-            uint32_t r[32];
-            tmem_ld32(lanes + (uint32_t)(F::BUFS * BN + c), r);
-            tc::tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              acc[c + j] += fmaf(acc[c + j], kUnitLoss, __uint_as_float(r[j]));
-          }
-          release(cross_empty);
+          for (int c = 0; c < COLS / 2; ++c) acc[c] = fma2(acc[c], loss, acc[c]);
         }
         if (g.split > 1) {
           float* part = stages_f + (q * 32 + lane) * F::PART_PITCH + half * COLS;
 #pragma unroll
-          for (int c = 0; c < COLS; c += 4)
-            *reinterpret_cast<float4*>(part + c) =
-                make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+          for (int c = 0; c < COLS; c += 4) {
+            const float2 a = unpair(acc[c / 2]), b = unpair(acc[c / 2 + 1]);
+            *reinterpret_cast<float4*>(part + c) = make_float4(a.x, a.y, b.x, b.y);
+          }
           break;  // one tile a cluster: summed below
         }
 #pragma unroll
@@ -802,7 +715,11 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
           if (n0 + c >= g.N) break;
           float v[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = acc[c + j] * f;
+          for (int j = 0; j < 16; ++j) {
+            const float2 a = unpair(acc[c / 2 + j]);
+            v[2 * j] = a.x * f;
+            v[2 * j + 1] = a.y * f;
+          }
           finish32<I8>(g, v, T, m, n0 + c, stage, lane);
         }
       }
@@ -852,7 +769,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
           }
           if (!I8 && g.e.mode <= kEpiPoly) {
             uint32_t hi[4], lo[4];
-            terms8(g, v, T.b, m, n, hi, lo);
+            terms8(g, v, T.b, m, n, linear8(g, 0, T.b, m, n), linear8(g, 1, T.b, m, n), hi, lo);
           } else if (I8 && g.e.mode == kEpiPlanes) {
             const GemmEpiArgs& e = g.e;
             const int pixel = e.m_base + m, img = pixel / e.pixels, px = pixel - img * e.pixels;

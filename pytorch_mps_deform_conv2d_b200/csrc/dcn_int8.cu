@@ -4,11 +4,16 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "dcn_dense_common.cuh"
 #include "dcn_launch.h"
 
 namespace dcn {
 
 namespace {
+
+using dense::fma2;
+using dense::pair;
+using dense::unpair;
 
 template <int T>
 __device__ __forceinline__ float ld(const void* p, long long i) {
@@ -216,22 +221,6 @@ sample_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ of
   if (lane == 0) scale[(long long)gi * np + lp] = s;
 }
 
-// Two fp32 values side by side, and a multiply-add of both at once.
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 __device__ __forceinline__ float max_abs_nan(float top, float v) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(v)));

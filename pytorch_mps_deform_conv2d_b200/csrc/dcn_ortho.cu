@@ -26,6 +26,7 @@
 #include <cuda_fp16.h>
 
 #include "dcn_capi_util.h"
+#include "dcn_ortho_chain.h"
 
 namespace dcn {
 
@@ -312,7 +313,25 @@ cudaError_t launch_ortho(const OrthoShape& s, const OrthoChunk& c, void* workspa
     e = product("ortho_gram", X, X, l.m, l.m, l.n, q, true);
     if (e != cudaSuccess) return e;
     unsigned short* prod = nullptr;  // Q so far
-    for (int i = 0; i < run; ++i) {
+    if (l.m <= kChainMax) {  // the run's products in one launch
+      ChainArgs a;
+      a.m = l.m;
+      a.run = run;
+      for (int i = 0; i < 3 * run; ++i) a.coef[i] = s.coef[3 * k + i];
+      a.scale_s = kScaleS;
+      a.scale_p = kScaleP;
+      a.scale_q = kScaleQ;
+      a.out = prod = Q[0];
+      a.pitch = l.spitch;
+      a.term_stride = l.sterm;
+      a.batch_stride = 2 * l.sterm;
+      *stage = "ortho_chain";
+      capi::ProfScope scope(*stage, stream);
+      e = launch_ortho_chain(a, square(S), c.count, wait_limit, no_async, stream);
+      scope.done();
+      if (e != cudaSuccess) return e;
+    }
+    for (int i = 0; l.m > kChainMax && i < run; ++i) {
       const float* abc = s.coef + 3 * (k + i);
       unsigned short* poly = prod == nullptr ? Q[0] : P;
       const float to = prod == nullptr ? kScaleQ : kScaleP;
@@ -335,7 +354,7 @@ cudaError_t launch_ortho(const OrthoShape& s, const OrthoChunk& c, void* workspa
         prod = poly;
       } else {
         unsigned short* next = prod == Q[0] ? Q[1] : Q[0];
-        e = product("ortho_chain", square(poly), square(prod), l.m, l.m, l.m,
+        e = product("ortho_join", square(poly), square(prod), l.m, l.m, l.m,
                     to_square(next, 1.f / to), true);
         if (e != cudaSuccess) return e;
         prod = next;
