@@ -129,8 +129,7 @@ __device__ __forceinline__ void split2(uint64_t v, uint32_t& hi, uint32_t& lo) {
   const float2 f = unpair(v);
   hi = pack2<kF16T>(f.x, f.y);
   const float2 h = unpack2<kF16T>(hi);
-  const float2 r = unpair(fma2(pair(h.x, h.y), pair(-1.f, -1.f), v));
-  lo = pack2<kF16T>(r.x, r.y);
+  lo = pack2<kF16T>(f.x - h.x, f.y - h.y);
 }
 // Two fp16 terms of a pair added up.
 __device__ __forceinline__ uint64_t join2(uint32_t hi, uint32_t lo) {

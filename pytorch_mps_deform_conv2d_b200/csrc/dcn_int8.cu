@@ -41,13 +41,25 @@ __device__ __forceinline__ int code_of(float v, float scale, bool usable) {
 }
 __device__ __forceinline__ bool usable_scale(float s) { return s > 0.f && s <= 3.402823466e38f; }
 
+// Rows of any length and alignment: the first 256 * KEEP values of a row wait
+// in registers for their scale.
 template <int T>
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const void* __restrict__ x, int cols, long long ldx,
                      signed char* __restrict__ q, long long ldq, float* __restrict__ scale) {
+  constexpr int KEEP = 8;
   const long long row = blockIdx.x;
+  float v[KEEP];
   unsigned top = 0;
-  for (int c = threadIdx.x; c < cols; c += 256) top = max(top, abs_bits(ld<T>(x, row * ldx + c)));
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k) {
+    const int c = threadIdx.x + 256 * k;
+    v[k] = c < cols ? ld<T>(x, row * ldx + c) : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k) top = max(top, abs_bits(v[k]));
+  for (int c = threadIdx.x + 256 * KEEP; c < cols; c += 256)
+    top = max(top, abs_bits(ld<T>(x, row * ldx + c)));
   __shared__ unsigned red[8];
   top = __reduce_max_sync(0xffffffffu, top);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
@@ -56,7 +68,12 @@ quantize_rows_kernel(const void* __restrict__ x, int cols, long long ldx,
   const float s = scale_of(top);
   const bool ok = usable_scale(s);
   if (threadIdx.x == 0) scale[row] = s;
-  for (int c = threadIdx.x; c < cols; c += 256)
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k) {
+    const int c = threadIdx.x + 256 * k;
+    if (c < cols) q[row * ldq + c] = (signed char)code_of(v[k], s, ok);
+  }
+  for (int c = threadIdx.x + 256 * KEEP; c < cols; c += 256)
     q[row * ldq + c] = (signed char)code_of(ld<T>(x, row * ldx + c), s, ok);
 }
 
@@ -141,14 +158,34 @@ quantize_rows8_kernel(const void* __restrict__ x, int vecs, long long ldx,
   }
 }
 
+// A warp a row: 16 bytes a lane from wherever the row starts (two aligned
+// words around each), 16-byte stores.
 __global__ void __launch_bounds__(256)
 repack_i8_kernel(const signed char* __restrict__ in, long long rows, int cols,
                  signed char* __restrict__ out, long long ldo) {
-  const long long n = rows * cols;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n;
-       i += (long long)gridDim.x * 256) {
-    const long long r = i / cols;
-    out[r * ldo + (i - r * cols)] = in[i];
+  const int lane = threadIdx.x & 31;
+  const long long total = rows * cols;
+  for (long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows;
+       r += (long long)gridDim.x * 8) {
+    const long long at = r * cols;
+    const uintptr_t start = reinterpret_cast<uintptr_t>(in + at);
+    const uint32_t* word = reinterpret_cast<const uint32_t*>(start & ~(uintptr_t)3);
+    const int shift = (int)(start & 3) * 8;
+    // words that begin before the end of the matrix may be read whole: they
+    // share an aligned word with a byte of it
+    const long long left = (total - at + (start & 3) + 3) / 4;
+    for (int c = 16 * lane; c < cols; c += 512) {
+      uint32_t w[5];
+#pragma unroll
+      for (int j = 0; j < 5; ++j) w[j] = c / 4 + j < left ? __ldg(word + c / 4 + j) : 0u;
+      uint4 v;
+      v.x = __funnelshift_r(w[0], w[1], shift);
+      v.y = __funnelshift_r(w[1], w[2], shift);
+      v.z = __funnelshift_r(w[2], w[3], shift);
+      v.w = __funnelshift_r(w[3], w[4], shift);
+      // (what follows the row's end in its last 16 bytes is never read)
+      *reinterpret_cast<uint4*>(out + r * ldo + c) = v;
+    }
   }
 }
 
@@ -435,16 +472,31 @@ few_tokens_kernel(const void* __restrict__ x, const float* __restrict__ x_scale,
     for (int t = 0; t < NT; ++t) scale[t] = t < tokens ? __ldg(x_scale + t) : 0.f;
     __syncthreads();
   } else {
+    // the first 8 * 256 * KEEP values of a token wait in registers
+    constexpr int KEEP = NT == 1 ? 2 : NT == 2 ? 1 : 0;
+    float v[NT][KEEP > 0 ? KEEP : 1][8];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       unsigned top = 0;
-      if (t < tokens)
-        for (int c = tid; c < K / 8; c += 256) {
-          float v[8];
-          ld8<T>(x, (long long)t * K + 8LL * c, v);
+      auto take = [&](const float(&u)[8]) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[j]));
+        for (int j = 0; j < 8; ++j) top = max(top, abs_bits(u[j]));
+      };
+      if (t < tokens) {
+#pragma unroll
+        for (int k = 0; k < KEEP; ++k) {
+          const int c = tid + 256 * k;
+          if (c < K / 8) {
+            ld8<T>(x, (long long)t * K + 8LL * c, v[t][k]);
+            take(v[t][k]);
+          }
         }
+        for (int c = tid + 256 * KEEP; c < K / 8; c += 256) {
+          float u[8];
+          ld8<T>(x, (long long)t * K + 8LL * c, u);
+          take(u);
+        }
+      }
       top = __reduce_max_sync(0xffffffffu, top);
       if (lane == 0) red[t][warp] = top;
     }
@@ -458,10 +510,19 @@ few_tokens_kernel(const void* __restrict__ x, const float* __restrict__ x_scale,
       const bool ok = usable_scale(s);
       scale[t] = s;
       uint2* dst = reinterpret_cast<uint2*>(xq + (long long)t * vecs);
-      for (int c = tid; c < K / 8; c += 256) {
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (t < tokens) ld8<T>(x, (long long)t * K + 8LL * c, v);
-        dst[c] = codes8(v, s, ok);
+      if (t < tokens) {
+#pragma unroll
+        for (int k = 0; k < KEEP; ++k) {
+          const int c = tid + 256 * k;
+          if (c < K / 8) dst[c] = codes8(v[t][k], s, ok);
+        }
+        for (int c = tid + 256 * KEEP; c < K / 8; c += 256) {
+          float u[8];
+          ld8<T>(x, (long long)t * K + 8LL * c, u);
+          dst[c] = codes8(u, s, ok);
+        }
+      } else {
+        for (int c = tid; c < K / 8; c += 256) dst[c] = make_uint2(0, 0);
       }
     }
     __syncthreads();
@@ -615,8 +676,8 @@ cudaError_t launch_few_tokens(const void* x, int x_type, const float* x_scale, i
 
 cudaError_t launch_repack_i8(const signed char* in, long long rows, int cols, signed char* out,
                              long long ldo, cudaStream_t stream) {
-  const long long n = rows * cols, blocks = (n + 255) / 256;
-  if (n <= 0) return cudaSuccess;
+  const long long blocks = (rows + 7) / 8;
+  if (rows <= 0 || cols <= 0) return cudaSuccess;
   repack_i8_kernel<<<(unsigned)(blocks < 2368 ? blocks : 2368), 256, 0, stream>>>(in, rows, cols,
                                                                                  out, ldo);
   return cudaGetLastError();

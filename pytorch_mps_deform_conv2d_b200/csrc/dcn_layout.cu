@@ -214,6 +214,46 @@ __global__ void __launch_bounds__(256) transpose16_kernel(const unsigned short* 
   }
 }
 
+// The same in 64 x 64 tiles with 8-byte loads and stores, for R and S multiples
+// of 4 and 8-byte aligned buffers: four times fewer memory instructions (the
+// neck's (2, 256, 15200) 16.8 -> 8.5 us with the launch).
+__global__ void __launch_bounds__(256)
+transpose16x4_kernel(const unsigned short* __restrict__ in, unsigned short* __restrict__ out,
+                     int R, int S, unsigned short* tail, int tail_n) {
+  __shared__ unsigned short tile[64][66];
+  if (tail != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0)
+    for (int i = threadIdx.x; i < tail_n; i += 256) tail[i] = 0;
+  const long long image = (long long)blockIdx.z * R * S;
+  const int r0 = blockIdx.y * 64, s0 = blockIdx.x * 64;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  uint2 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = r0 + ty + 16 * i, s = s0 + tx * 4;
+    v[i] = make_uint2(0, 0);
+    if (r < R && s < S)
+      v[i] = *reinterpret_cast<const uint2*>(in + image + (long long)r * S + s);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {  // rows of 132 bytes: 4-byte stores
+    uint32_t* t = reinterpret_cast<uint32_t*>(&tile[ty + 16 * i][tx * 4]);
+    t[0] = v[i].x;
+    t[1] = v[i].y;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int s = s0 + ty + 16 * i, r = r0 + tx * 4;
+    if (s < S && r < R) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = tile[tx * 4 + j][ty + 16 * i];
+      *reinterpret_cast<uint2*>(out + image + (long long)s * R + r) =
+          make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+    }
+  }
+}
+
 // 16-bit (bf16, or fp16 with `f16`) <-> fp32, element-wise; fp32 -> 16-bit
 // rounds to nearest even.
 __global__ void h16_to_f32_kernel(const unsigned short* __restrict__ in, float* __restrict__ out,
@@ -241,6 +281,12 @@ cudaError_t launch_nchw_to_nhwc_bf16(const void* x, void* xt, int N, int C, int 
     return cudaSuccess;
   }
   if (ceil_div(C, 32) > 65535 || N > 65535) return cudaErrorInvalidValue;
+  if (C % 4 == 0 && HW % 4 == 0 &&
+      ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(xt)) & 7) == 0) {
+    transpose16x4_kernel<<<dim3(ceil_div(HW, 64), ceil_div(C, 64), N), 256, 0, stream>>>(
+        static_cast<const unsigned short*>(x), out, C, HW, tail, C);
+    return cudaGetLastError();
+  }
   dim3 grid(ceil_div(HW, 32), ceil_div(C, 32), N);
   transpose16_kernel<<<grid, dim3(32, 8), 0, stream>>>(static_cast<const unsigned short*>(x), out,
                                                        C, HW, tail, C);

@@ -22,10 +22,9 @@
 // times fp32 products or below them; one run of five steps diverges.
 #include "dcn_ortho.h"
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include "dcn_capi_util.h"
+#include "dcn_dense_common.cuh"
+#include "dcn_launch.h"
 #include "dcn_ortho_chain.h"
 
 namespace dcn {
@@ -36,7 +35,7 @@ namespace {
 // in a run of the usual steps, 8 at most), P (its coefficients, 16 at most),
 // Q (products of at most 150^(1/2) with room for 256).
 constexpr float kScaleS = 8192.f, kScaleP = 4096.f, kScaleQ = 256.f;
-constexpr int kPartials = 64;  // sums of squares a matrix
+constexpr int kPartials = 256;  // sums of squares a matrix, at most
 constexpr float kRunLimit = 150.f, kFirstRunLimit = 12.f;
 
 struct PrepArgs {
@@ -48,33 +47,77 @@ struct PrepArgs {
   unsigned short* x;
   long long numel, pitch, term_stride, batch_stride;
   int rows, cols, type, terms, target;  // |stored X| lies in [2^target, 2^(target + 1))
-  int muon, nesterov;
+  int muon, nesterov, vec, partials;
   float beta, eps;
 };
 
-__device__ __forceinline__ float load_in(const PrepArgs& a, int b, long long i) {
-  const void* p = a.in[b];
-  if (a.type == kF32) return static_cast<const float*>(p)[i];
-  if (a.type == kBF16T) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  return __half2float(static_cast<const __half*>(p)[i]);
+template <int T>
+__device__ __forceinline__ float load1(const void* p, long long i) {
+  if constexpr (T == kF32) return static_cast<const float*>(p)[i];
+  else if constexpr (T == kBF16T)
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  else return __half2float(static_cast<const __half*>(p)[i]);
+}
+// Eight values from i, a multiple of eight behind a 16-byte aligned pointer.
+template <int T>
+__device__ __forceinline__ void load8(const void* p, long long i, float (&v)[8]) {
+  if constexpr (T == kF32) {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const float4 a = q[0], b = q[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+    const uint4 a =
+        *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(p) + i);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = dense::unpack2<T>(w[j]);
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
+  }
 }
 
-// The update's value at i from the new momentum.
+// The update's value from the gradient and the new momentum.
 __device__ __forceinline__ float update_of(const PrepArgs& a, float g, float m) {
   return a.nesterov ? (1.f - a.beta) * g + a.beta * m : m;
 }
 
 // New momentum, and sums of squares of the update in 64 bits: any fp32 input
-// keeps its norm, and the partial sums' fixed order keeps the result.
+// keeps its norm, and the partial sums' fixed order keeps the result.  Bound
+// by HBM (a step reads the gradient, reads and writes the momentum).
+template <int T>
 __global__ void __launch_bounds__(256) ortho_norm_kernel(const __grid_constant__ PrepArgs a) {
   const int b = blockIdx.y;
+  const void* in = a.in[b];
+  float* mom = a.momentum[b];
+  const long long step = (long long)gridDim.x * 256;
+  const long long first = (long long)blockIdx.x * 256 + threadIdx.x;
   double s = 0.0;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.numel;
-       i += (long long)kPartials * 256) {
-    float v = load_in(a, b, i);
+  const long long vecs = a.vec ? a.numel / 8 : 0;
+  for (long long q = first; q < vecs; q += step) {
+    float v[8];
+    load8<T>(in, 8 * q, v);
     if (a.muon) {
-      const float m = a.beta * a.momentum[b][i] + (1.f - a.beta) * v;
-      a.momentum[b][i] = m;
+      float m[8];
+      load8<kF32>(mom, 8 * q, m);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m[j] = a.beta * m[j] + (1.f - a.beta) * v[j];
+      float4* o = reinterpret_cast<float4*>(mom + 8 * q);
+      o[0] = make_float4(m[0], m[1], m[2], m[3]);
+      o[1] = make_float4(m[4], m[5], m[6], m[7]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = update_of(a, v[j], m[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += (double)v[j] * (double)v[j];
+  }
+  for (long long i = 8 * vecs + first; i < a.numel; i += step) {
+    float v = load1<T>(in, i);
+    if (a.muon) {
+      const float m = a.beta * mom[i] + (1.f - a.beta) * v;
+      mom[i] = m;
       v = update_of(a, v, m);
     }
     s += (double)v * (double)v;
@@ -92,49 +135,69 @@ __global__ void __launch_bounds__(256) ortho_norm_kernel(const __grid_constant__
 // X as fp16 terms of the update times a power of two: exact for 16-bit inputs
 // (but for what lies 2^-24 below the largest), and 1 / (norm + eps) is left to
 // the products' epilogues in fp32.
+template <int T>
 __global__ void __launch_bounds__(256) ortho_scale_kernel(const __grid_constant__ PrepArgs a) {
   const int b = blockIdx.y;
   __shared__ float f1, f2;
-  if (threadIdx.x == 0) {
+  dense::grid_launch_dependents();
+  dense::grid_wait();
+  if (threadIdx.x < 32) {
     double s = 0.0;
-    for (int i = 0; i < kPartials; ++i) s += a.partial[b * kPartials + i];
-    const double norm = sqrt(s);
-    int k = 0;
-    if (norm > 0.0 && isfinite(norm)) k = a.target - ilogb(norm);
-    f1 = (float)ldexp(1.0, k / 2);
-    f2 = (float)ldexp(1.0, k - k / 2);
-    if (blockIdx.x == 0) {
-      // a norm that is not finite leaves nothing to scale by
-      const float r = isfinite(norm) ? (float)ldexp(1.0 / (norm + (double)a.eps), -k)
-                                     : __int_as_float(0x7fc00000);
-      a.r1[b] = r;
-      a.r2[b] = r * r;
+    for (int i = threadIdx.x; i < a.partials; i += 32) s += a.partial[b * kPartials + i];
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (threadIdx.x == 0) {
+      const double norm = sqrt(s);
+      int k = 0;
+      if (norm > 0.0 && isfinite(norm)) k = a.target - ilogb(norm);
+      f1 = (float)ldexp(1.0, k / 2);
+      f2 = (float)ldexp(1.0, k - k / 2);
+      if (blockIdx.x == 0) {
+        // a norm that is not finite leaves nothing to scale by
+        const float r = isfinite(norm) ? (float)ldexp(1.0 / (norm + (double)a.eps), -k)
+                                       : __int_as_float(0x7fc00000);
+        a.r1[b] = r;
+        a.r2[b] = r * r;
+      }
     }
   }
   __syncthreads();
+  const void* in = a.in[b];
+  const float* mom = a.momentum[b];
+  const float c1 = f1, c2 = f2;
   const int chunks = (int)(a.pitch / 8);
+  const bool vec = a.vec && a.cols % 8 == 0;
   const long long total = (long long)a.rows * chunks;
   for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < total;
        q += (long long)gridDim.x * 256) {
     const int row = (int)(q / chunks), c = (int)(q - (long long)row * chunks) * 8;
-    __align__(16) unsigned short hi[8], lo[8];
+    const long long i = (long long)row * a.cols + c;
+    float v[8];
+    if (vec) {
+      load8<T>(in, i, v);
+      if (a.muon) {
+        float m[8];
+        load8<kF32>(mom, i, m);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float v = 0.f;
-      if (c + j < a.cols) {
-        const long long i = (long long)row * a.cols + c + j;
-        v = load_in(a, b, i);
-        if (a.muon) v = update_of(a, v, a.momentum[b][i]);
-        v = v * f1 * f2;
+        for (int j = 0; j < 8; ++j) v[j] = update_of(a, v[j], m[j]);
       }
-      const __half h = __float2half_rn(v);
-      hi[j] = __half_as_ushort(h);
-      lo[j] = __half_as_ushort(__float2half_rn(v - __half2float(h)));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = 0.f;
+        if (c + j < a.cols) {
+          v[j] = load1<T>(in, i + j);
+          if (a.muon) v[j] = update_of(a, v[j], mom[i + j]);
+        }
+      }
     }
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      dense::split2(dense::pair(v[2 * j] * c1 * c2, v[2 * j + 1] * c1 * c2), hi[j], lo[j]);
     unsigned short* x = a.x + (long long)b * a.batch_stride + (long long)row * a.pitch + c;
-    *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(hi);
+    *reinterpret_cast<uint4*>(x) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     if (a.terms == 2)
-      *reinterpret_cast<uint4*>(x + a.term_stride) = *reinterpret_cast<const uint4*>(lo);
+      *reinterpret_cast<uint4*>(x + a.term_stride) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
 }
 
@@ -249,19 +312,41 @@ cudaError_t launch_ortho(const OrthoShape& s, const OrthoChunk& c, void* workspa
   p.nesterov = c.nesterov;
   p.beta = c.beta;
   p.eps = s.eps;
+  p.vec = 1;
+  for (int i = 0; i < c.count; ++i)
+    if ((reinterpret_cast<uintptr_t>(c.in[i]) | reinterpret_cast<uintptr_t>(c.momentum[i])) & 15)
+      p.vec = 0;
+  // 4096 values a block at least, and some eight blocks an SM over all matrices
+  long long parts = (p.numel + 4095) / 4096;
+  const long long most = (8LL * device_sm_count() + c.count - 1) / c.count;
+  if (parts > most) parts = most;
+  p.partials = (int)(parts < kPartials ? parts : kPartials);
   *stage = "ortho_norm";
+  auto norm = s.type == kF32 ? ortho_norm_kernel<kF32>
+              : s.type == kBF16T ? ortho_norm_kernel<kBF16T> : ortho_norm_kernel<kF16T>;
   capi::ProfScope norm_scope(*stage, stream);
-  ortho_norm_kernel<<<dim3(kPartials, c.count), 256, 0, stream>>>(p);
+  norm<<<dim3(p.partials, c.count), 256, 0, stream>>>(p);
   norm_scope.done();
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   *stage = "ortho_scale";
   const long long chunks = s.rows * (l.xpitch / 8);
-  const long long blocks = (chunks + 255) / 256;
+  long long blocks = (chunks + 511) / 512;
+  if (blocks > most) blocks = most;
+  auto scale = s.type == kF32 ? ortho_scale_kernel<kF32>
+               : s.type == kBF16T ? ortho_scale_kernel<kBF16T> : ortho_scale_kernel<kF16T>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks, (unsigned)c.count);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   capi::ProfScope scale_scope(*stage, stream);
-  ortho_scale_kernel<<<dim3((unsigned)(blocks < 592 ? blocks : 592), c.count), 256, 0, stream>>>(p);
+  e = cudaLaunchKernelEx(&cfg, scale, p);
   scale_scope.done();
-  e = cudaGetLastError();
   if (e != cudaSuccess) return e;
 
   auto square = [&](const unsigned short* base) {

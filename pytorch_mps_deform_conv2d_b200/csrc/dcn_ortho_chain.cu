@@ -178,33 +178,35 @@ ortho_chain_kernel(const __grid_constant__ CUtensorMap smap, const __grid_consta
       // the last result goes to global memory
       unsigned char* dst = i + 1 == ops ? nullptr
                            : op.kind == kS ? S : op.kind == kQ || op.step == 0 ? Q : P;
-      uint64_t acc[2][16];
-#pragma unroll 1
-      for (int u = 0; u < units; ++u) {
-        ok = wait_warp(watch, &acc_full[u], i & 1);
-        if (!ok) break;
-        tc::tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          if (64 * c + 32 * h >= cols) continue;
-          uint32_t r[32];
-          tmem_ld32(tmem + lanes + u * N + 64 * c + 32 * h, r);
-          tc::tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const uint64_t x = pair(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-            acc[c][j] = u == 0 ? x : add2(acc[c][j], x);
-          }
-        }
-      }
+      // the last unit's commit covers the products of all
+      ok = wait_warp(watch, &acc_full[units - 1], i & 1);
       if (!ok) break;
+      tc::tc_fence_after();
       // (the rows from `cols` on are nobody's operand and hold anything)
       const uint64_t loss = pair(kUnitLoss, kUnitLoss), f2 = pair(factor, factor);
       const uint64_t cb2 = pair(cb, cb);
       if (q * 32 < cols) {
+#pragma unroll 1
+        for (int c0 = 32 * h; c0 < cols; c0 += 64) {
+          uint64_t acc[16];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int c0 = 64 * c + 32 * h;
+          for (int u = 0; u < UNITS; u += 2) {  // two units' columns at a time
+            if (u >= units) continue;
+            uint32_t r[2][32];
+            tmem_ld32(tmem + lanes + u * N + c0, r[0]);
+            if (u + 1 < units) tmem_ld32(tmem + lanes + (u + 1) * N + c0, r[1]);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+              if (u + v >= units) continue;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const uint64_t x =
+                    pair(__uint_as_float(r[v][2 * e]), __uint_as_float(r[v][2 * e + 1]));
+                acc[e] = u + v == 0 ? x : add2(acc[e], x);
+              }
+            }
+          }
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
             const int col = c0 + j;
@@ -212,7 +214,7 @@ ortho_chain_kernel(const __grid_constant__ CUtensorMap smap, const __grid_consta
             uint64_t v[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const uint64_t x = acc[c][j / 2 + e];
+              const uint64_t x = acc[j / 2 + e];
               v[e] = mul2(fma2(x, loss, x), f2);
             }
             if (poly) {  // + b S + a I
