@@ -473,7 +473,7 @@ few_tokens_kernel(const void* __restrict__ x, const float* __restrict__ x_scale,
     __syncthreads();
   } else {
     // the first 8 * 256 * KEEP values of a token wait in registers
-    constexpr int KEEP = NT == 1 ? 2 : NT == 2 ? 1 : 0;
+    constexpr int KEEP = 0;
     float v[NT][KEEP > 0 ? KEEP : 1][8];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
