@@ -300,7 +300,9 @@ __device__ __forceinline__ uint64_t raw_pair(const Raw8<T>& r, int j) {
 // Channels in eights (per group, per deformable group).  WPP warps share an
 // item, so that each lane holds at most NV vectors of eight samples in
 // registers from the gather to their codes: the input is gathered once and
-// only codes are written.  The sampling plans of an item (corner offsets,
+// only codes are written.  What counts is bytes on their way: at most five
+// vectors a lane, so that three blocks fit an SM, and the corners of one
+// vector fetched while the last one's are used (the neck's 100 -> @N us).  The sampling plans of an item (corner offsets,
 // weights with the mask) are made once, a lane each, in shared memory; then
 // lane l takes vectors l, l + 32 WPP, ... of the column.  Bound by the L2 -> SM
 // traffic of the corners (four of 16 bytes for eight codes).
@@ -310,7 +312,7 @@ struct alignas(16) PlanI8 {
 };
 
 template <int T, int NV>
-__global__ void __launch_bounds__(256, NV <= 3 ? 4 : 2)
+__global__ void __launch_bounds__(256, 3)
 sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ off,
                   const void* __restrict__ mask, long long p0, int np,
                   signed char* __restrict__ col, int kp, float* __restrict__ scale, int wpp,
@@ -358,28 +360,45 @@ sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ o
   const long long img = (long long)n * g.HW * g.C;
   uint64_t v[NV][4];  // pairs of fp32
   float top = 0.f;    // NaN stays
+  // (tap, vector of the tap) of the lane's next vector, and their step
+  const int start = part * 32 + lane, stride = 32 * wpp;
+  int k = start / cvec, cv = start - k * cvec;
+  const int dk = stride / cvec, dc = stride - dk * cvec;
+  // the next vector's corners are on their way while the last one's are used
+  Raw8<T> raw[2][4];
+  float w[2][4];
+  auto fetch = [&](int i) {
+    const bool any = start + i * stride < nvec;
+    const int ch = gi * g.Cg + cv * 8;
+    const PlanI8 q = mine[any ? k * gdg + (gdg > 1 ? ch / g.cpg - dg0 : 0) : 0];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      raw[i & 1][c] = ld8_if<T>(x, img + q.at[c] + ch, any && q.at[c] >= 0);
+      w[i & 1][c] = q.w[c];
+    }
+    k += dk;
+    cv += dc;
+    if (cv >= cvec) {
+      cv -= cvec;
+      ++k;
+    }
+  };
+  fetch(0);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
+    if (i + 1 < NV) fetch(i + 1);
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[i][j] = 0;
-    const int idx = part * 32 + lane + i * 32 * wpp;
-    if (idx < nvec) {
-      const int k = idx / cvec, ch = gi * g.Cg + (idx - k * cvec) * 8;
-      const PlanI8 q = mine[k * gdg + (gdg > 1 ? ch / g.cpg - dg0 : 0)];
-      Raw8<T> raw[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) raw[c] = ld8_if<T>(x, img + q.at[c] + ch, q.at[c] >= 0);
+    for (int c = 0; c < 4; ++c) {
+      const uint64_t w2 = pair(w[i & 1][c], w[i & 1][c]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint64_t w2 = pair(q.w[c], q.w[c]);
+      for (int j = 0; j < 4; ++j) v[i][j] = fma2(raw_pair<T>(raw[i & 1][c], j), w2, v[i][j]);
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[i][j] = fma2(raw_pair<T>(raw[c], j), w2, v[i][j]);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = unpair(v[i][j]);
-        top = max_abs_nan(max_abs_nan(top, f.x), f.y);
-      }
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpair(v[i][j]);
+      top = max_abs_nan(max_abs_nan(top, f.x), f.y);
     }
   }
   unsigned bits = __reduce_max_sync(0xffffffffu, abs_bits(top));
@@ -454,6 +473,18 @@ few_tokens_kernel(const void* __restrict__ x, const float* __restrict__ x_scale,
   const int vecs = K / 16;
   const int row0 = (blockIdx.x * 8 + warp) * ROWS;
   constexpr int AHEAD = kFewAhead / ROWS;
+  // the first 8 * 256 * KEEP values of each token are asked for before the
+  // weight is, or they would wait for it
+  constexpr int KEEP = T == 3 || NT > 2 ? 0 : 2 / NT;
+  Raw8<T == 3 ? 0 : T> raw[NT][KEEP > 0 ? KEEP : 1];
+  if constexpr (KEEP > 0) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int k = 0; k < KEEP; ++k)
+        raw[t][k] = ld8_if<T>(x, (long long)t * K + 8LL * (tid + 256 * k),
+                              t < tokens && tid + 256 * k < K / 8);
+  }
   uint4 wv[ROWS][AHEAD];
   const uint4* wr[ROWS];
 #pragma unroll
@@ -472,9 +503,14 @@ few_tokens_kernel(const void* __restrict__ x, const float* __restrict__ x_scale,
     for (int t = 0; t < NT; ++t) scale[t] = t < tokens ? __ldg(x_scale + t) : 0.f;
     __syncthreads();
   } else {
-    // the first 8 * 256 * KEEP values of a token wait in registers
-    constexpr int KEEP = 0;
-    float v[NT][KEEP > 0 ? KEEP : 1][8];
+    auto kept = [&](int t, int k, float(&v)[8]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = unpair(raw_pair<T>(raw[t][k], j));
+        v[2 * j] = f.x;
+        v[2 * j + 1] = f.y;
+      }
+    };
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       unsigned top = 0;
@@ -485,11 +521,9 @@ few_tokens_kernel(const void* __restrict__ x, const float* __restrict__ x_scale,
       if (t < tokens) {
 #pragma unroll
         for (int k = 0; k < KEEP; ++k) {
-          const int c = tid + 256 * k;
-          if (c < K / 8) {
-            ld8<T>(x, (long long)t * K + 8LL * c, v[t][k]);
-            take(v[t][k]);
-          }
+          float u[8];
+          kept(t, k, u);
+          take(u);
         }
         for (int c = tid + 256 * KEEP; c < K / 8; c += 256) {
           float u[8];
@@ -514,7 +548,9 @@ few_tokens_kernel(const void* __restrict__ x, const float* __restrict__ x_scale,
 #pragma unroll
         for (int k = 0; k < KEEP; ++k) {
           const int c = tid + 256 * k;
-          if (c < K / 8) dst[c] = codes8(v[t][k], s, ok);
+          float u[8];
+          kept(t, k, u);
+          if (c < K / 8) dst[c] = codes8(u, s, ok);
         }
         for (int c = tid + 256 * KEEP; c < K / 8; c += 256) {
           float u[8];
@@ -609,14 +645,14 @@ cudaError_t sample_type(const Geom& g, const void* x, const void* off, const voi
   const int gdg = g.Cg >= g.cpg ? g.Cg / g.cpg : 1;
   const bool nested = g.Cg % g.cpg == 0 || g.cpg % g.Cg == 0;
   const long long nvec = (long long)g.kk * g.Cg / 8;
-  if (g.Cg % 8 == 0 && g.cpg % 8 == 0 && nested && nvec <= 9 * 32 * 8 &&
+  if (g.Cg % 8 == 0 && g.cpg % 8 == 0 && nested && nvec <= 5 * 32 * 8 &&
       (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
       sizeof(PlanI8) * g.kk * gdg * 8 <= 96 * 1024) {
     int wpp = 1;
-    while (nvec > 9LL * 32 * wpp) wpp *= 2;
+    while (nvec > 5LL * 32 * wpp) wpp *= 2;
     const long long nv = (nvec + 32 * wpp - 1) / (32 * wpp);
     auto form = nv <= 1 ? sample8_form<T, 1> : nv <= 3 ? sample8_form<T, 3>
-                : nv <= 5 ? sample8_form<T, 5> : sample8_form<T, 9>;
+                : sample8_form<T, 5>;
     return form(g, x, off, mask, p0, np, col, kp, scale, wpp, gdg, stream);
   }
   const size_t one = (size_t)g.kk * g.Cg * sizeof(float);
