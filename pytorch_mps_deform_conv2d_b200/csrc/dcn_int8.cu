@@ -298,14 +298,15 @@ __device__ __forceinline__ uint64_t raw_pair(const Raw8<T>& r, int j) {
 }
 
 // Channels in eights (per group, per deformable group).  WPP warps share an
-// item, so that each lane holds at most NV vectors of eight samples in
-// registers from the gather to their codes: the input is gathered once and
-// only codes are written.  What counts is bytes on their way: at most five
-// vectors a lane, so that three blocks fit an SM, and the corners of one
-// vector fetched while the last one's are used (the neck's 100 -> @N us).  The sampling plans of an item (corner offsets,
-// weights with the mask) are made once, a lane each, in shared memory; then
-// lane l takes vectors l, l + 32 WPP, ... of the column.  Bound by the L2 -> SM
-// traffic of the corners (four of 16 bytes for eight codes).
+// item (a pixel and group), so that each lane holds at most NV vectors of eight
+// samples in registers from the gather to their codes: the input is gathered
+// once and only codes are written.  A block first makes the sampling plans
+// (corner offsets, weights with the mask) of all its items in shared memory,
+// neighbouring lanes on neighbouring pixels; then its warps work through the
+// items without waiting for one another, the corners of one vector on their
+// way while the last one's are used.  Bound by the L2 -> SM traffic of the
+// corners (four of 16 bytes for eight codes) and its latency: with the plans
+// made item by item the neck's columns took 100 us, like this @N.
 struct alignas(16) PlanI8 {
   int at[4];  // element offsets of the corners within the image
   float w[4];
@@ -316,47 +317,52 @@ __global__ void __launch_bounds__(256, 3)
 sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ off,
                   const void* __restrict__ mask, long long p0, int np,
                   signed char* __restrict__ col, int kp, float* __restrict__ scale, int wpp,
-                  int gdg) {
-  extern __shared__ PlanI8 plans[];
-  __shared__ unsigned red[8];
+                  int gdg, int ib) {
+  extern __shared__ PlanI8 plans[];  // [npl][ib]
+  __shared__ unsigned red[2][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slot = warp / wpp, part = warp - slot * wpp, slots = 8 / wpp;
-  const long long item = (long long)blockIdx.x * slots + slot;
-  const bool live = item < (long long)np * g.G;
-  const int gi = live ? (int)(item / np) : 0, lp = live ? (int)(item - (long long)gi * np) : 0;
-  const long long pix = p0 + lp;
-  const int n = (int)(pix / g.P), p = (int)(pix - (long long)n * g.P);
-  const int oy = p / g.Wo, ox = p - oy * g.Wo;
-  const int dg0 = gi * g.Cg / g.cpg;  // the group's first deformable group; gdg of them
-  PlanI8* mine = plans + slot * g.kk * gdg;
-  if (live) {
-    for (int i = part * 32 + lane; i < g.kk * gdg; i += wpp * 32) {
-      const int k = i / gdg, dgi = dg0 + i - k * gdg;
-      const int ki = k / g.kw, kj = k - ki * g.kw;
-      const long long oi = off_h_index(g, n, dgi, k, p);
-      float h, w;
-      sample_pos(g, oy, ox, ki, kj, ld<T>(off, oi), ld<T>(off, oi + g.P), h, w);
-      float m = 1.f;
-      if (g.use_mask) {
-        m = ld<T>(mask, mask_index(g, n, dgi, k, p));
-        if (g.mask_logits) m = 1.f / (1.f + expf(-m));
-      }
-      const Sample sp = make_sample(h, w, g.H, g.W);
-      PlanI8 q;
-      // a dropped corner: offset -1, not read
-      q.at[0] = sp.live & 1u ? sp.i1 * g.C : -1;
-      q.at[1] = sp.live & 2u ? sp.i2 * g.C : -1;
-      q.at[2] = sp.live & 4u ? sp.i3 * g.C : -1;
-      q.at[3] = sp.live & 8u ? sp.i4 * g.C : -1;
-      q.w[0] = sp.w1 * m;
-      q.w[1] = sp.w2 * m;
-      q.w[2] = sp.w3 * m;
-      q.w[3] = sp.w4 * m;
-      mine[i] = q;
+  const long long first = (long long)blockIdx.x * ib, items = (long long)np * g.G;
+  const int mine = (int)min((long long)ib, items - first), npl = g.kk * gdg;
+  for (int i = threadIdx.x; i < ib * npl; i += 256) {
+    const int pl = i / ib, it = i - pl * ib;
+    if (it >= mine) continue;
+    const long long item = first + it;
+    const int gi = (int)(item / np);
+    const long long pix = p0 + (item - (long long)gi * np);
+    const int n = (int)(pix / g.P), p = (int)(pix - (long long)n * g.P);
+    const int oy = p / g.Wo, ox = p - oy * g.Wo;
+    const int k = pl / gdg, dgi = gi * g.Cg / g.cpg + pl - k * gdg;
+    const int ki = k / g.kw, kj = k - ki * g.kw;
+    const long long oi = off_h_index(g, n, dgi, k, p);
+    float h, w;
+    sample_pos(g, oy, ox, ki, kj, ld<T>(off, oi), ld<T>(off, oi + g.P), h, w);
+    float m = 1.f;
+    if (g.use_mask) {
+      m = ld<T>(mask, mask_index(g, n, dgi, k, p));
+      if (g.mask_logits) m = 1.f / (1.f + expf(-m));
     }
+    const Sample sp = make_sample(h, w, g.H, g.W);
+    PlanI8 q;
+    // a dropped corner: offset -1, not read
+    q.at[0] = sp.live & 1u ? sp.i1 * g.C : -1;
+    q.at[1] = sp.live & 2u ? sp.i2 * g.C : -1;
+    q.at[2] = sp.live & 4u ? sp.i3 * g.C : -1;
+    q.at[3] = sp.live & 8u ? sp.i4 * g.C : -1;
+    q.w[0] = sp.w1 * m;
+    q.w[1] = sp.w2 * m;
+    q.w[2] = sp.w3 * m;
+    q.w[3] = sp.w4 * m;
+    plans[i] = q;
   }
   __syncthreads();
-  const int cvec = g.Cg / 8, nvec = live ? g.kk * cvec : 0;
+  const int cvec = g.Cg / 8, nvec = g.kk * cvec;
+  int turn = 0;
+#pragma unroll 1
+  for (int it = slot; it < mine; it += slots, turn ^= 1) {
+  const long long item = first + it;
+  const int gi = (int)(item / np), lp = (int)(item - (long long)gi * np);
+  const int n = (int)((p0 + lp) / g.P), dg0 = gi * g.Cg / g.cpg;
   const long long img = (long long)n * g.HW * g.C;
   uint64_t v[NV][4];  // pairs of fp32
   float top = 0.f;    // NaN stays
@@ -370,7 +376,7 @@ sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ o
   auto fetch = [&](int i) {
     const bool any = start + i * stride < nvec;
     const int ch = gi * g.Cg + cv * 8;
-    const PlanI8 q = mine[any ? k * gdg + (gdg > 1 ? ch / g.cpg - dg0 : 0) : 0];
+    const PlanI8 q = plans[(any ? k * gdg + (gdg > 1 ? ch / g.cpg - dg0 : 0) : 0) * ib + it];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       raw[i & 1][c] = ld8_if<T>(x, img + q.at[c] + ch, any && q.at[c] >= 0);
@@ -403,11 +409,10 @@ sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ o
   }
   unsigned bits = __reduce_max_sync(0xffffffffu, abs_bits(top));
   if (wpp > 1) {  // the item's warps agree on its largest value
-    if (lane == 0) red[warp] = bits;
-    __syncthreads();
-    for (int w = 0; w < wpp; ++w) bits = max(bits, red[slot * wpp + w]);
+    if (lane == 0) red[turn][warp] = bits;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "r"(32 * wpp) : "memory");
+    for (int o = 0; o < wpp; ++o) bits = max(bits, red[turn][slot * wpp + o]);
   }
-  if (!live) return;
   const float s = scale_of(bits);
   const bool ok = usable_scale(s);
   // one reciprocal for the item: the samples are rounded sums already, so the
@@ -435,6 +440,7 @@ sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ o
     }
   }
   if (part == 0 && lane == 0) scale[(long long)gi * np + lp] = s;
+  }
 }
 
 template <int T, int NV>
@@ -443,12 +449,18 @@ cudaError_t sample8_form(const Geom& g, const void* x, const void* off, const vo
                          int gdg, cudaStream_t stream) {
   const long long items = (long long)np * g.G;
   const int slots = 8 / wpp;
-  const size_t smem = sizeof(PlanI8) * g.kk * gdg * slots;
+  // items a block: 32, fewer where their plans would take more than 32 KB or
+  // the blocks would not fill the SMs three times over
+  const int one = (int)sizeof(PlanI8) * g.kk * gdg;
+  int ib = 32;
+  while (ib > slots && (ib * one > 32 * 1024 || items < (long long)ib * 3 * device_sm_count()))
+    ib /= 2;
+  const int smem = one * ib;
   auto kern = sample8_i8_kernel<T, NV>;
-  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), (int)smem);
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
-  kern<<<(unsigned)((items + slots - 1) / slots), 256, smem, stream>>>(
-      g, x, off, mask, p0, np, col, kp, scale, wpp, gdg);
+  kern<<<(unsigned)((items + ib - 1) / ib), 256, smem, stream>>>(
+      g, x, off, mask, p0, np, col, kp, scale, wpp, gdg, ib);
   return cudaGetLastError();
 }
 
