@@ -432,6 +432,8 @@ DCN_API int dcn_deform_int8(const dcn_shape* shape, int type, const void* input,
     q.epi.pixels = g.P;
     q.epi.channels = g.outC;
     q.epi.m_base = (int)p0;
+    q.epi.pixel_pairs = np % 2 == 0 && p0 % 2 == 0 && g.P % 2 == 0 &&
+                        (reinterpret_cast<uintptr_t>(output) & 3) == 0;
     q.wait_limit = g.wait_limit;
     q.no_async = g.no_async;
     DCN_CUDA(dcn::launch_gemm(q, stream), "int8_gemm");

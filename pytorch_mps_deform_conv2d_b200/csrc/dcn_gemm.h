@@ -67,7 +67,8 @@ struct GemmEpiArgs {
   const void* bias;  // of out_type's sibling `bias_type`
   int bias_type;
   int pixels, channels;  // kEpiPlanes: pixels an image, channels of all groups,
-  int m_base;            // and the pixel that m = 0 stands for
+  int m_base;            // and the pixel that m = 0 stands for; pixel_pairs:
+  int pixel_pairs;       // M, m_base and pixels are even, `out` 4-byte aligned
   void* list[kGemmMaxList];
 };
 

@@ -402,6 +402,23 @@ __device__ __forceinline__ void planes32(const GemmArgs& g, const float (&v)[32]
   if (m >= g.M) return;
   const int pixel = e.m_base + m, img = pixel / e.pixels, px = pixel - img * e.pixels;
   const long long at = ((long long)img * e.channels + (long long)b * g.N + n0) * e.pixels + px;
+  if constexpr (T != kF32) {
+    // Pixels in pairs (both of one image, both < M): lanes 2 i and 2 i + 1
+    // trade a value, the even one stores channel c of both pixels, the odd one
+    // channel c + 1
+    if (e.pixel_pairs) {
+      const bool odd = pixel & 1;
+      unsigned short* out = static_cast<unsigned short*>(e.out) + (odd ? at - 1 + e.pixels : at);
+#pragma unroll
+      for (int c = 0; c < 32; c += 2) {
+        const float other = __shfl_xor_sync(__activemask(), odd ? v[c] : v[c + 1], 1);
+        const uint32_t w = odd ? pack2<T>(other, v[c + 1]) : pack2<T>(v[c], other);
+        if (n0 + c + odd < g.N)
+          *reinterpret_cast<uint32_t*>(out + (long long)c * e.pixels) = w;
+      }
+      return;
+    }
+  }
 #pragma unroll
   for (int c = 0; c < 32; ++c)
     if (n0 + c < g.N) store_f<T>(e.out, at + (long long)c * e.pixels, v[c]);

@@ -305,15 +305,15 @@ __device__ __forceinline__ uint64_t raw_pair(const Raw8<T>& r, int j) {
 // neighbouring lanes on neighbouring pixels; then its warps work through the
 // items without waiting for one another, the corners of one vector on their
 // way while the last one's are used.  Bound by the L2 -> SM traffic of the
-// corners (four of 16 bytes for eight codes) and its latency: with the plans
-// made item by item the neck's columns took 100 us, like this @N.
+// corners (four of 16 bytes for eight codes): the neck's columns in 77 us, 7.3
+// TB/s of corners (100 us with the plans made item by item).
 struct alignas(16) PlanI8 {
   int at[4];  // element offsets of the corners within the image
   float w[4];
 };
 
 template <int T, int NV>
-__global__ void __launch_bounds__(256, 3)
+__global__ void __launch_bounds__(256, NV > 5 ? 2 : 3)
 sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ off,
                   const void* __restrict__ mask, long long p0, int np,
                   signed char* __restrict__ col, int kp, float* __restrict__ scale, int wpp,
@@ -660,11 +660,15 @@ cudaError_t sample_type(const Geom& g, const void* x, const void* off, const voi
   if (g.Cg % 8 == 0 && g.cpg % 8 == 0 && nested && nvec <= 5 * 32 * 8 &&
       (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
       sizeof(PlanI8) * g.kk * gdg * 8 <= 96 * 1024) {
+    // one warp an item up to nine vectors a lane (no warp waits for another:
+    // neck 89 -> 81 us), else several with five at most (three blocks an SM
+    // instead of two: the 512-channel sweep 95 us against 99)
     int wpp = 1;
-    while (nvec > 5LL * 32 * wpp) wpp *= 2;
+    if (nvec > 9 * 32)
+      while (nvec > 5LL * 32 * wpp) wpp *= 2;
     const long long nv = (nvec + 32 * wpp - 1) / (32 * wpp);
     auto form = nv <= 1 ? sample8_form<T, 1> : nv <= 3 ? sample8_form<T, 3>
-                : sample8_form<T, 5>;
+                : nv <= 5 ? sample8_form<T, 5> : sample8_form<T, 9>;
     return form(g, x, off, mask, p0, np, col, kp, scale, wpp, gdg, stream);
   }
   const size_t one = (size_t)g.kk * g.Cg * sizeof(float);
