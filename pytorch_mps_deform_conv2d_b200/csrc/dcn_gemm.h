@@ -78,6 +78,7 @@ struct GemmProblem {
   int a_batch_mod;  // batch index of A is b % a_batch_mod (0: b)
   bool int8, sym;
   bool fine;        // two-term operands: sums to fp32's accuracy
+  bool coarse;      // results of 11 bits and less
   bool after_ours;  // the launch before is one of this library's products, or
                     // another kernel whose writes this one may wait for late
   GemmEpiArgs epi;

@@ -28,7 +28,10 @@
 // warps add the units in registers, rounding to nearest.  For fp32 results
 // units of 32 values, the cross terms (2^-11 as large, and so are their losses)
 // before hi hi; what is lost on average, 1.1 units of 2^-24 (0.8 for terms of
-// both signs, 1.4 for squares), is added back.  For 16-bit results units of 256.
+// both signs, 1.4 for squares), is added back.  For 16-bit results units of 256, for
+// those of 11 bits and less units of 1024 where tensor memory is busiest (a
+// drain of 256 columns takes it from the products: 4096 x 4096 x 4096 126 us in
+// units of 256, 98 us whole; a sum of 1024 loses 6e-6 of its size).
 #pragma once
 
 #include "dcn_dense_common.cuh"
@@ -887,8 +890,11 @@ cudaError_t launch_tiling(const GemmProblem& p, cudaStream_t stream) {
   auto tiles = [&](int tm, int tn) {
     return (long long)((p.M + tm - 1) / tm) * ((p.N + tn - 1) / tn) * p.batch;
   };
-  if (tiles(256, 256) * 2 >= sms)
+  if (tiles(256, 256) * 2 >= sms) {
+    if constexpr (UNIT == 16 && TA + TB < 4)
+      if (p.coarse) return launch_form<I8, TA, TB, AT, BT, 256, 64, true>(p, 1, stream);
     return launch_form<I8, TA, TB, AT, BT, 256, UNIT, true>(p, 1, stream);
+  }
   if (tiles(128, 128) >= sms)
     return launch_form<I8, TA, TB, AT, BT, 128, UNIT, false>(p, 1, stream);
   const int ksteps = (p.K + (I8 ? 127 : 63)) / (I8 ? 128 : 64);

@@ -370,6 +370,7 @@ cudaError_t launch_ortho(const OrthoShape& s, const OrthoChunk& c, void* workspa
     g.batch = c.count;
     g.sym = sym;
     g.fine = s.type == kF32;
+    g.coarse = s.later_terms == 1;
     g.after_ours = true;
     g.epi = epi;
     g.wait_limit = wait_limit;
