@@ -15,11 +15,11 @@
 // those values grow.  A run ends before the product of its a^2 passes 150:
 // three steps of the usual 3.4445, two runs for five steps; results of 16 bits
 // do not see the difference.  For fp32 results the first run, where one
-// direction can hold nearly all of |X|, ends before 12: two steps, then three.
-// Emulated in 64 bits on 64 x 576 with a few strong directions, the relative
-// error is 5e-7 with (2, 3) and 4.6e-6 with (3, 2), fp32 products as written
-// 1.4e-6; over flat, power-law and exponential spectra (2, 3) stays within 1.6
-// times fp32 products or below them; one run of five steps diverges.
+// direction can hold nearly all of |X|, ends before 12: two steps; so does
+// every run of more than 256 directions.  Emulated in 64 bits on 64 x 576 with
+// a few strong directions, the relative error is 5e-7 with runs (2, 3) and
+// 4.6e-6 with (3, 2), fp32 products as written 1.4e-6; one run of five steps
+// diverges on steep spectra.
 #include "dcn_ortho.h"
 
 #include "dcn_capi_util.h"
@@ -36,7 +36,7 @@ namespace {
 // Q (products of at most 150^(1/2) with room for 256).
 constexpr float kScaleS = 8192.f, kScaleP = 4096.f, kScaleQ = 256.f;
 constexpr int kPartials = 256;  // sums of squares a matrix, at most
-constexpr float kRunLimit = 150.f, kFirstRunLimit = 12.f;
+constexpr float kRunLimit = 150.f, kShortRunLimit = 12.f;
 
 struct PrepArgs {
   const void* in[kGemmMaxList];
@@ -241,7 +241,11 @@ int run_length(const OrthoShape& s, int first) {
   const int m = s.rows < s.cols ? s.rows : s.cols, n = s.rows < s.cols ? s.cols : s.rows;
   if (m > kChainMax && n < 2 * m && (first > 0 || s.later_terms == 2)) return 1;
   const bool f32 = s.first_terms == 2 && s.later_terms == 2;
-  const float limit = first == 0 && f32 ? kFirstRunLimit : kRunLimit;
+  // The more directions, the more of them are still small in the second run.
+  // Relative errors with runs (2, 3), (2, 2, 1) and of fp32 products: 300 x 2700
+  // 0.85e-6, 1.0e-6, 1.5e-6; 515 x 1153 3.2e-6, 2.0e-6, 2.6e-6; 1400 x 2900
+  // 6.7e-6, 2.7e-6, 3.8e-6.
+  const float limit = f32 && (first == 0 || m > 256) ? kShortRunLimit : kRunLimit;
   float grown = 1.f;
   int k = first;
   while (k + 1 < s.steps) {
