@@ -717,7 +717,8 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
         }
         if (!ok) break;
         if constexpr (UNIT == 2) {
-          const uint64_t loss = pair(kUnitLoss, kUnitLoss);
+          const float lost = g.K <= 16 ? kStepLoss : kUnitLoss;
+          const uint64_t loss = pair(lost, lost);
 #pragma unroll
           for (int c = 0; c < COLS / 2; ++c) acc[c] = fma2(acc[c], loss, acc[c]);
         }

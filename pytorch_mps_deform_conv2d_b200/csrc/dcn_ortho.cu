@@ -241,11 +241,13 @@ int run_length(const OrthoShape& s, int first) {
   const int m = s.rows < s.cols ? s.rows : s.cols, n = s.rows < s.cols ? s.cols : s.rows;
   if (m > kChainMax && n < 2 * m && (first > 0 || s.later_terms == 2)) return 1;
   const bool f32 = s.first_terms == 2 && s.later_terms == 2;
-  // The more directions, the more of them are still small in the second run.
+  // The more directions, and the squarer the matrix, the more of them are still
+  // small in the second run.
   // Relative errors with runs (2, 3), (2, 2, 1) and of fp32 products: 300 x 2700
   // 0.85e-6, 1.0e-6, 1.5e-6; 515 x 1153 3.2e-6, 2.0e-6, 2.6e-6; 1400 x 2900
   // 6.7e-6, 2.7e-6, 3.8e-6.
-  const float limit = f32 && (first == 0 || m > 256) ? kShortRunLimit : kRunLimit;
+  const float limit =
+      f32 && (first == 0 || m > 256 || n < 2 * m) ? kShortRunLimit : kRunLimit;
   float grown = 1.f;
   int k = first;
   while (k + 1 < s.steps) {

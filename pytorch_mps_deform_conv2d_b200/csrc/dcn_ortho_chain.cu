@@ -183,7 +183,8 @@ ortho_chain_kernel(const __grid_constant__ CUtensorMap smap, const __grid_consta
       if (!ok) break;
       tc::tc_fence_after();
       // (the rows from `cols` on are nobody's operand and hold anything)
-      const uint64_t loss = pair(kUnitLoss, kUnitLoss), f2 = pair(factor, factor);
+      const float lost = ksteps == 1 ? kStepLoss : kUnitLoss;
+      const uint64_t loss = pair(lost, lost), f2 = pair(factor, factor);
       const uint64_t cb2 = pair(cb, cb);
       if (q * 32 < cols) {
 #pragma unroll 1
