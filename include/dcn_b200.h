@@ -332,8 +332,10 @@ DCN_API int dcn_h16_staging(const dcn_shape* shape, uint32_t flags);
  * on the tensor cores: float32 matrices keep fp32 accuracy (two fp16 terms an
  * operand), or that of one TF32 product with DCN_MATH_TF32 in `flags`; 16-bit
  * matrices keep what their type can hold.  A matrix with NaN or an infinity
- * gives NaN everywhere.  At most 32 steps, 2^31 - 1 elements and a smaller
- * side of 32768. */
+ * gives NaN everywhere.  Made for polynomials that keep singular values of
+ * [0, 1] below 2: S is held up to 8, a I + b S + c S S up to 16; beyond, results
+ * may be NaN.  At most 32 steps, coefficients of 15, 2^31 - 1 elements and a
+ * smaller side of 32768. */
 DCN_API size_t dcn_newton_schulz_workspace_size(int64_t count, int64_t rows, int64_t cols,
                                                 int type, int steps, uint32_t flags);
 DCN_API int dcn_newton_schulz(int64_t count, int64_t rows, int64_t cols, int type,

@@ -102,6 +102,8 @@ int deform_int8_plan(const dcn_shape* shape, int type, uint32_t flags, DeformInt
   DCN_CHECK(float_type(type), "%s: input, offset and mask must be float32, bfloat16 or float16",
             op);
   const dcn::Geom& g = d.g;
+  if (!(flags & DCN_INPUT_NHWC) && g.N > 65535)
+    return fail(DCN_ERR_UNSUPPORTED, "%s: more than 65535 NCHW images are not supported", op);
   d.kg = (int64_t)g.Cg * g.kk;
   if (d.kg > kInt8MaxK)
     return fail(DCN_ERR_UNSUPPORTED, "%s: more than %lld columns a group are not supported", op,

@@ -57,8 +57,7 @@ struct GemmEpiArgs {
   const unsigned short* lin16;
   int out_terms;
   long long pitch, term_stride, batch_stride;
-  void* out;            // base of matrix 0, or NULL: `list`
-  long long out_batch;  // elements from one matrix to the next
+  void* out;  // NULL: list[matrix]
   int out_type;
   int wide_ok;  // rows of `out` take 16-byte stores
   const float* row_scale;
@@ -75,7 +74,6 @@ struct GemmEpiArgs {
 struct GemmProblem {
   GemmOperand a, b;  // D[m, n] = sum_k A[m, k] B[n, k]
   int M, N, K, batch;
-  int a_batch_mod;  // batch index of A is b % a_batch_mod (0: b)
   bool int8, sym;
   bool fine;        // two-term operands: sums to fp32's accuracy
   bool coarse;      // results of 11 bits and less

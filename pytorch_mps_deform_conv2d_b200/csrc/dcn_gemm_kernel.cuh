@@ -58,7 +58,7 @@ constexpr int kMiscBytes = 1024 + 256 + 2048 + EPI_WARPS * kStageWarp;
 
 struct GemmArgs {
   int M, N, K;
-  int a_mod, a_shared, b_shared;
+  int a_shared, b_shared;
   int mt, nt, per_batch, tiles;  // tiles: mt x nt, or the upper triangle of them
   int sym;
   int split;  // CTAs of a cluster that share a tile's K
@@ -266,9 +266,8 @@ __device__ __forceinline__ void terms8(const GemmArgs& g, const float (&v)[8], i
         make_uint4(lo[0], lo[1], lo[2], lo[3]);
 }
 
-__device__ __forceinline__ void* out_base(const GemmEpiArgs& e, int b, int es) {
-  return e.out != nullptr ? static_cast<char*>(e.out) + (long long)b * e.out_batch * es
-                          : e.list[b];
+__device__ __forceinline__ void* out_base(const GemmEpiArgs& e, int b) {
+  return e.out != nullptr ? e.out : e.list[b];
 }
 
 // Dense rows of N, 16-byte stores (N and the base allow them; N % 8 == 0 is not
@@ -444,7 +443,7 @@ __device__ __forceinline__ void finish32(const GemmArgs& g, float (&v)[32], cons
       return;
     }
   }
-  void* base = out_base(g.e, T.b, type == kF32 ? 4 : 2);
+  void* base = out_base(g.e, T.b);
   if (type == kF32) rows32<kF32>(g, v, base, m, n0, stage, lane);
   else if (type == kBF16T) rows32<kBF16T>(g, v, base, m, n0, stage, lane);
   else rows32<kF16T>(g, v, base, m, n0, stage, lane);
@@ -514,7 +513,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
       bool ok = true;
       for (int t = first_tile; t < g.tiles && ok; t += tile_step) {
         const Tile T = tile_of<F, PAIR>(g, t, rank);
-        const int ba = g.a_shared ? 0 : (g.a_mod ? T.b % g.a_mod : T.b);
+        const int ba = g.a_shared ? 0 : T.b;
         const int bb = g.b_shared ? 0 : T.b;
         const int bn0 = T.n0 + (PAIR ? rank * F::BROWS : 0);
         for (int k = k0; k < k1; ++k, ++it) {
@@ -805,7 +804,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
               else store_f<kF16T>(e.out, at1, v[j]);
             }
           } else {
-            void* base = out_base(g.e, T.b, g.e.out_type == kF32 ? 4 : 2);
+            void* base = out_base(g.e, T.b);
             if (g.e.out_type == kF32) rows8<kF32>(g, v, base, m, n);
             else if (g.e.out_type == kBF16T) rows8<kBF16T>(g, v, base, m, n);
             else rows8<kF16T>(g, v, base, m, n);
@@ -835,7 +834,6 @@ cudaError_t launch_form(const GemmProblem& p, int split, cudaStream_t stream) {
   g.M = p.M;
   g.N = p.N;
   g.K = p.K;
-  g.a_mod = p.a_batch_mod;
   g.a_shared = p.a.batch == 1;
   g.b_shared = p.b.batch == 1;
   g.mt = (p.M + F::TM - 1) / F::TM;

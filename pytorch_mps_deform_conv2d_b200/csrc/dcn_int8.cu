@@ -349,10 +349,11 @@ sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ o
     q.at[1] = sp.live & 2u ? sp.i2 * g.C : -1;
     q.at[2] = sp.live & 4u ? sp.i3 * g.C : -1;
     q.at[3] = sp.live & 8u ? sp.i4 * g.C : -1;
-    q.w[0] = sp.w1 * m;
-    q.w[1] = sp.w2 * m;
-    q.w[2] = sp.w3 * m;
-    q.w[3] = sp.w4 * m;
+    // (nor weighted: a mask that is not finite must not reach it)
+    q.w[0] = sp.live & 1u ? sp.w1 * m : 0.f;
+    q.w[1] = sp.live & 2u ? sp.w2 * m : 0.f;
+    q.w[2] = sp.live & 4u ? sp.w3 * m : 0.f;
+    q.w[3] = sp.live & 8u ? sp.w4 * m : 0.f;
     plans[i] = q;
   }
   __syncthreads();
@@ -417,7 +418,10 @@ sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ o
   const bool ok = usable_scale(s);
   // one reciprocal for the item: the samples are rounded sums already, so the
   // codes are within those roundings of the formula's
-  const float inv = ok ? 1.f / s : 0.f;
+  // (a scale whose reciprocal could overflow divides; one that is not usable
+  // gives zeros)
+  const bool fast = ok && s > 1e-35f;
+  const float inv = fast ? 1.f / s : 0.f;
   signed char* out = col + ((long long)gi * np + lp) * kp;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -435,7 +439,16 @@ sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ o
       uint2 c;
       c.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
       c.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
-      if (!ok) c = make_uint2(0, 0);
+      if (!fast) {
+        float u[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = unpair(v[i][j]);
+          u[2 * j] = f.x;
+          u[2 * j + 1] = f.y;
+        }
+        c = codes8(u, s, ok);
+      }
       *reinterpret_cast<uint2*>(out + 8 * idx) = c;
     }
   }

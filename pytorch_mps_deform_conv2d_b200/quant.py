@@ -110,6 +110,14 @@ class Int8DeformConv2d(nn.Module):
                    module.dilation, module.conv_offset if pack else None,
                    module.deformable_groups if pack else 1, module.modulated if pack else True)
 
+    def _apply(self, fn, *args, **kwargs):
+        # .half() and the like leave the scales in float32
+        scale = self.weight_scale
+        super()._apply(fn, *args, **kwargs)
+        if self.weight_scale.dtype != scale.dtype:
+            self.weight_scale = scale.to(self.weight_scale.device)
+        return self
+
     @torch.no_grad()
     def forward(self, input: Tensor, offset: Optional[Tensor] = None,
                 mask: Optional[Tensor] = None,

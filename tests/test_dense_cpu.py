@@ -113,7 +113,18 @@ def test_deform_int8_c_refusals():
     assert call(n=16) == WORKSPACE and call(x=None) == INVALID and call(t=I8) == INVALID
     assert call(ot=I8) == INVALID and call(stride_h=0) == INVALID and call(groups=3) == INVALID
     assert call(in_channels=20000) == UNSUPPORTED  # 180000 columns a group
+    assert call(batch=65536) == UNSUPPORTED
     assert call(batch=0) == OK
+
+
+def test_int8_module_keeps_its_scales_in_float32():
+    m = dcn.Int8DeformConv2d(torch.zeros(4, 2, 3, 3, dtype=torch.int8), torch.rand(4),
+                             torch.rand(4), 1, 1, 1)
+    scale = m.weight_scale.clone()
+    m = m.half()
+    assert m.weight.dtype == torch.int8 and m.bias.dtype == torch.float16
+    assert m.weight_scale.dtype == torch.float32 and torch.equal(m.weight_scale, scale)
+    assert set(m.state_dict()) == {"weight", "weight_scale", "bias"}
 
 
 def meta(*shape, dtype=torch.float32):

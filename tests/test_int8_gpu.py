@@ -239,6 +239,59 @@ def test_deform_far_offsets_and_values_that_are_not_finite(cuda_device):
     assert y[0].isfinite().all() and y[1, :, 4, 4].isnan().all() and y[1, :, 8, 8].isfinite().all()
 
 
+@pytest.mark.parametrize("c", [16, 5])
+def test_deform_values_at_the_edges_of_the_range(cuda_device, c):
+    # columns whose scale is below the normal range, and masks that are not
+    # finite where nothing is sampled
+    k = deform_case(c=c, o=8, bias=False)
+    small = {**k, "x": k["x"] * 1e-38}
+    assert rel(run_deform(small).double() * 1e30, ref_deform(small) * 1e30) <= 2e-2
+    far = {**k, "off": torch.full_like(k["off"], 1e6),
+           "mask": torch.full_like(k["mask"], float("nan"))}
+    assert not run_deform(far).any()
+
+
+def test_deform_in_several_chunks_of_pixels(cuda_device):
+    # 2 x 78400 pixels of 2304 codes: more than are kept at a time.  Pixels do
+    # not depend on one another: image by image gives the same bits
+    k = deform_case(n=2, c=256, h=280, w=280, o=40, dtype=torch.bfloat16)
+    y = run_deform(k)
+    for i in range(2):
+        one = {**k, **{t: k[t][i:i + 1] for t in ("x", "off", "mask")}}
+        assert torch.equal(run_deform(one)[0], y[i])
+
+
+def test_one_dimensional_token(cuda_device):
+    x, w, s = torch.randn(64, device="cuda"), rand_codes(24, 64), torch.rand(24, device="cuda")
+    assert torch.equal(dcn.int8_linear(x, w, s), dcn.int8_linear(x[None], w, s)[0])
+    q, xs = dcn.quantize_int8(x)
+    assert xs.shape == () and torch.equal(dcn.int8_linear(q, w, s, x_scale=xs),
+                                          dcn.int8_linear(x, w, s))
+
+
+def test_operators_under_compile_and_opcheck(cuda_device):
+    x, w, s = torch.randn(6, 64, device="cuda"), rand_codes(24, 64), torch.rand(24, device="cuda")
+    k = deform_case()
+
+    def all_of(x):
+        q, xs = dcn.quantize_int8(x)
+        return (dcn.int8_linear(x, w, s), dcn.int8_linear(q, w, s, x_scale=xs),
+                dcn.newton_schulz(x), run_deform(k))
+
+    for a, b in zip(torch.compile(all_of, fullgraph=True, backend="aot_eager")(x), all_of(x)):
+        assert torch.equal(a, b)
+    ops = _native.load_ops()
+    tests = ("test_schema", "test_faketensor")
+    torch.library.opcheck(ops.quantize_int8.default, (x,), test_utils=tests)
+    torch.library.opcheck(ops.int8_linear.default, (x, w, s), test_utils=tests)
+    torch.library.opcheck(ops.newton_schulz.default, (x, 5, [3.4445, -4.775, 2.0315], 1e-7),
+                          test_utils=tests)
+    p, g, m = (torch.randn(8, 16, device="cuda") for _ in range(3))
+    torch.library.opcheck(ops.muon_update_.default,
+                          ([p], [g], [m], 0.1, 0.9, True, 0.0, 5, [3.4445, -4.775, 2.0315], 1e-7),
+                          test_utils=tests)
+
+
 def test_deform_refusals_and_empty(cuda_device):
     k = deform_case()
     for change, match in ((dict(off=k["off"][:, :, 1:]), "offset shape"),
