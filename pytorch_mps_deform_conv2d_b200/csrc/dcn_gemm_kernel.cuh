@@ -11,9 +11,9 @@
 //            of what a 128 x 128 tile takes.  L2 -> SM loads are what bounds
 //            large products (about 70 bytes a nanosecond and SM, measured);
 //   128 x 128 where pairs would leave SMs idle;
-//   128 x 64  for small products, K split over a cluster of up to eight CTAs,
-//            whose partial sums meet in distributed shared memory: with few
-//            tiles the time is that of one SM's loads.
+//   128 x 64 and 64 x 64 for small products, K split over a cluster of up to
+//            eight CTAs, whose partial sums meet in distributed shared memory:
+//            with few tiles the time is that of one SM's loads.
 //
 // fp16 operands of two terms, x = hi + lo with lo = fp16(x - hi), carry 22
 // bits.  A K slice brings both terms of both operands once and the tensor core
@@ -48,7 +48,6 @@ using namespace dense;
 
 __device__ int g_gemm_status = 0;
 
-constexpr int BM = 128;
 constexpr int EPI_WARP0 = 2, EPI_WARPS = 8;
 constexpr int THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
 constexpr int kSmemMax = 227 * 1024;
@@ -68,12 +67,13 @@ struct GemmArgs {
 };
 
 // I8: int8 operands.  TA, TB: terms.  AT, BT: the operand's rows run along K.
-// UNIT: K of a unit in steps of 16 (0: all of K, int32 sums are exact).  PAIR:
-// two CTAs a tile.
-template <bool I8, int TA, int TB, bool AT, bool BT, int BN, int UNIT, bool PAIR>
+// BM: rows of A in a CTA.  UNIT: K of a unit in steps of 16 (0: all of K, int32
+// sums are exact).  PAIR: two CTAs a tile.
+template <bool I8, int TA, int TB, bool AT, bool BT, int BM, int BN, int UNIT, bool PAIR>
 struct Form {
   static constexpr int BK = I8 ? 128 : 64;  // 128 bytes of K
   static constexpr int TM = PAIR ? 2 * BM : BM;     // rows of a tile
+  static constexpr int WROWS = BM / 4;              // rows in a quarter of the lanes
   static constexpr int BROWS = PAIR ? BN / 2 : BN;  // rows of B in this CTA
   static constexpr int A_TERM = BM * 128, B_TERM = BROWS * 128;
   static constexpr int STAGE = TA * A_TERM + TB * B_TERM;
@@ -157,6 +157,7 @@ __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
                : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();  // the barrier takes whole warps
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -203,7 +204,7 @@ __device__ __forceinline__ Tile tile_of(const GemmArgs& g, int t, int rank) {
     tn = tm + i;
     r.mirrored = tn != tm;
   }
-  r.m0 = tm * F::TM + (PAIR ? rank * BM : 0);
+  r.m0 = tm * F::TM + (PAIR ? rank * (F::TM / 2) : 0);
   r.n0 = tn * (F::COLS * 2);
   return r;
 }
@@ -368,7 +369,7 @@ __device__ __forceinline__ void terms32(const GemmArgs& g, float (&v)[32], const
 // buffer, so that its lanes write neighbouring columns.
 template <int T>
 __device__ __forceinline__ void rows32(const GemmArgs& g, const float (&v)[32], void* base, int m,
-                                       int n0, float* stage, int lane) {
+                                       int n0, float* stage, int lane, int first, int rows) {
   if (g.e.wide_ok) {
     if (m >= g.M) return;
 #pragma unroll
@@ -381,7 +382,6 @@ __device__ __forceinline__ void rows32(const GemmArgs& g, const float (&v)[32], 
     }
     return;
   }
-  const int first = m - lane, rows = min(32, g.M - first);
 #pragma unroll
   for (int h = 0; h < 32; h += 16) {  // 16 columns at a time, two rows a store
 #pragma unroll
@@ -428,7 +428,8 @@ __device__ __forceinline__ void planes32(const GemmArgs& g, const float (&v)[32]
 
 template <bool I8>
 __device__ __forceinline__ void finish32(const GemmArgs& g, float (&v)[32], const Tile& T, int m,
-                                         int n0, float* stage, int lane) {
+                                         int n0, float* stage, int lane, int first, int rows) {
+  // lanes hold rows m = first + lane, the first `rows` of them
   const int type = g.e.out_type;
   if constexpr (I8) {
     if (g.e.mode == kEpiPlanes) {
@@ -444,16 +445,16 @@ __device__ __forceinline__ void finish32(const GemmArgs& g, float (&v)[32], cons
     }
   }
   void* base = out_base(g.e, T.b);
-  if (type == kF32) rows32<kF32>(g, v, base, m, n0, stage, lane);
-  else if (type == kBF16T) rows32<kBF16T>(g, v, base, m, n0, stage, lane);
-  else rows32<kF16T>(g, v, base, m, n0, stage, lane);
+  if (type == kF32) rows32<kF32>(g, v, base, m, n0, stage, lane, first, rows);
+  else if (type == kBF16T) rows32<kBF16T>(g, v, base, m, n0, stage, lane, first, rows);
+  else rows32<kF16T>(g, v, base, m, n0, stage, lane, first, rows);
 }
 
-template <bool I8, int TA, int TB, bool AT, bool BT, int BN, int UNIT, bool PAIR>
+template <bool I8, int TA, int TB, bool AT, bool BT, int BM, int BN, int UNIT, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                const __grid_constant__ GemmArgs g) {
-  using F = Form<I8, TA, TB, AT, BT, BN, UNIT, PAIR>;
+  using F = Form<I8, TA, TB, AT, BT, BM, BN, UNIT, PAIR>;
   constexpr int STAGES = F::STAGES, COLS = F::COLS;
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = tc::smem_u32(smem_raw);
@@ -640,7 +641,9 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
     int n = 0, unit = 0;
     for (int t = first_tile; t < g.tiles; t += tile_step, ++n) {
       const Tile T = tile_of<F, PAIR>(g, t, rank);
-      const int m = T.m0 + q * 32 + lane, n0 = T.n0 + half * COLS;
+      // (64 rows of A lie in the first 16 lanes of each quarter)
+      const int first = T.m0 + q * F::WROWS, rows = min(F::WROWS, g.M - first);
+      const int m = lane < F::WROWS ? first + lane : g.M, n0 = T.n0 + half * COLS;
       if constexpr (I8) {
         const float rs = m < g.M ? __ldg(g.e.row_scale + T.b * g.e.row_scale_batch + m) : 0.f;
         // the epilogue warps alone: named barrier 1
@@ -660,17 +663,19 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
         ++unit;
         tc::tc_fence_after();
         if (g.split > 1) {
-          int* part = reinterpret_cast<int*>(stages_f) + (q * 32 + lane) * F::PART_PITCH +
-                      half * COLS;
+          int* part = reinterpret_cast<int*>(stages_f) +
+                      (q * F::WROWS + lane) * F::PART_PITCH + half * COLS;
 #pragma unroll 1
           for (int c = 0; c < COLS; c += 32) {
             uint32_t r[32];
             tmem_ld32(lanes + (uint32_t)(buf * BN + c), r);
             tc::tmem_ld_wait();
+            if (lane < F::WROWS) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4)
-              *reinterpret_cast<uint4*>(part + c + j) =
-                  make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+              for (int j = 0; j < 32; j += 4)
+                *reinterpret_cast<uint4*>(part + c + j) =
+                    make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+            }
           }
           break;  // one tile a cluster: summed below
         }
@@ -685,7 +690,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
             const float2 s = chan[half * COLS + c + j];
             v[j] = (float)(int)r[j] * rs * s.x + s.y;
           }
-          finish32<I8>(g, v, T, m, n0 + c, stage, lane);
+          finish32<I8>(g, v, T, m, n0 + c, stage, lane, first, rows);
         }
         release(&acc_empty[buf]);
       } else {
@@ -722,11 +727,13 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
           for (int c = 0; c < COLS / 2; ++c) acc[c] = fma2(acc[c], loss, acc[c]);
         }
         if (g.split > 1) {
-          float* part = stages_f + (q * 32 + lane) * F::PART_PITCH + half * COLS;
+          float* part = stages_f + (q * F::WROWS + lane) * F::PART_PITCH + half * COLS;
+          if (lane < F::WROWS) {
 #pragma unroll
-          for (int c = 0; c < COLS; c += 4) {
-            const float2 a = unpair(acc[c / 2]), b = unpair(acc[c / 2 + 1]);
-            *reinterpret_cast<float4*>(part + c) = make_float4(a.x, a.y, b.x, b.y);
+            for (int c = 0; c < COLS; c += 4) {
+              const float2 a = unpair(acc[c / 2]), b = unpair(acc[c / 2 + 1]);
+              *reinterpret_cast<float4*>(part + c) = make_float4(a.x, a.y, b.x, b.y);
+            }
           }
           break;  // one tile a cluster: summed below
         }
@@ -740,7 +747,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
             v[2 * j] = a.x * f;
             v[2 * j + 1] = a.y * f;
           }
-          finish32<I8>(g, v, T, m, n0 + c, stage, lane);
+          finish32<I8>(g, v, T, m, n0 + c, stage, lane, first, rows);
         }
       }
     }
@@ -827,9 +834,9 @@ inline cudaError_t make_map(CUtensorMap* map, const GemmOperand& o, bool int8, i
                       o.k_rows ? 64u : (uint32_t)box_rows);
 }
 
-template <bool I8, int TA, int TB, bool AT, bool BT, int BN, int UNIT, bool PAIR>
+template <bool I8, int TA, int TB, bool AT, bool BT, int BM, int BN, int UNIT, bool PAIR>
 cudaError_t launch_form(const GemmProblem& p, int split, cudaStream_t stream) {
-  using F = Form<I8, TA, TB, AT, BT, BN, UNIT, PAIR>;
+  using F = Form<I8, TA, TB, AT, BT, BM, BN, UNIT, PAIR>;
   GemmArgs g;
   g.M = p.M;
   g.N = p.N;
@@ -838,8 +845,9 @@ cudaError_t launch_form(const GemmProblem& p, int split, cudaStream_t stream) {
   g.b_shared = p.b.batch == 1;
   g.mt = (p.M + F::TM - 1) / F::TM;
   g.nt = (p.N + BN - 1) / BN;
-  // halves of a symmetric product only where the tiles are square
-  g.sym = p.sym && F::TM == BN;
+  // halves of a symmetric product only in large square tiles: small ones are
+  // there for their latency, and SMs are free
+  g.sym = p.sym && F::TM == BN && BN > 64;
   const long long per =
       g.sym ? (long long)g.nt * (g.nt + 1) / 2 : (long long)g.mt * g.nt;
   if (per * p.batch > (1LL << 29)) return cudaErrorInvalidValue;
@@ -853,7 +861,7 @@ cudaError_t launch_form(const GemmProblem& p, int split, cudaStream_t stream) {
   cudaError_t e = make_map(&amap, p.a, I8, BM);
   if (e == cudaSuccess) e = make_map(&bmap, p.b, I8, F::BROWS);
   if (e != cudaSuccess) return e;
-  auto kern = gemm_tc_kernel<I8, TA, TB, AT, BT, BN, UNIT, PAIR>;
+  auto kern = gemm_tc_kernel<I8, TA, TB, AT, BT, BM, BN, UNIT, PAIR>;
   e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), F::SMEM);
   if (e != cudaSuccess) return e;
   const int sms = device_sm_count();
@@ -891,26 +899,43 @@ cudaError_t launch_tiling(const GemmProblem& p, cudaStream_t stream) {
   };
   if (tiles(256, 256) * 2 >= sms) {
     if constexpr (UNIT == 16 && TA + TB < 4)
-      if (p.coarse) return launch_form<I8, TA, TB, AT, BT, 256, 64, true>(p, 1, stream);
-    return launch_form<I8, TA, TB, AT, BT, 256, UNIT, true>(p, 1, stream);
+      if (p.coarse) return launch_form<I8, TA, TB, AT, BT, 128, 256, 64, true>(p, 1, stream);
+    return launch_form<I8, TA, TB, AT, BT, 128, 256, UNIT, true>(p, 1, stream);
   }
   if (tiles(128, 128) >= sms)
-    return launch_form<I8, TA, TB, AT, BT, 128, UNIT, false>(p, 1, stream);
+    return launch_form<I8, TA, TB, AT, BT, 128, 128, UNIT, false>(p, 1, stream);
   const int ksteps = (p.K + (I8 ? 127 : 63)) / (I8 ? 128 : 64);
-  // K over a cluster: it costs some 2.5 us (its barriers, the partial sums'
-  // way) and saves K slices one after another, 0.28 us each, 0.65 of two-term
-  // operands to fp32's accuracy, 0.5 of others (measured, one to eight CTAs)
-  const double slice = TA + TB == 2 ? 0.28 : UNIT == 2 ? 0.65 : 0.5;
+  // Small products: the time of one CTA, K slices one after another (measured:
+  // one-term operands 0.26 us a slice in tiles of 64 x 64, 0.28 of 128 x 64;
+  // two-term ones 0.40 and 0.50, to fp32's accuracy 0.59 and 0.68).  K over a
+  // cluster divides the slices and costs 2.5 us (its barriers, the partial
+  // sums' way); of clusters of 4 and 8 no more than 32 and 14 fit the SMs'
+  // groups at a time.
+  const double slice64 = TA + TB == 2 ? 0.26 : UNIT == 2 ? 0.59 : 0.40;
+  const double slice128 = TA + TB == 2 ? 0.28 : UNIT == 2 ? 0.68 : 0.50;
+  const long long t64 = tiles(64, 64), t128 = tiles(128, 64);
+  double best = 1e30;
   int split = 1;
-  double best = slice * ksteps;
-  for (int s = 2; s <= 8 && tiles(128, 64) * s <= sms && s <= ksteps; s *= 2) {
-    const double cost = 2.5 + slice * ((ksteps + s - 1) / s);
-    if (cost < best) {
-      best = cost;
+  bool rows64 = false;
+  for (int s = 1; s <= 8 && s <= ksteps; s *= 2) {
+    const long long most = s == 1 ? sms : s == 2 ? sms / 2 : s == 4 ? 32 : 14;
+    const double fixed = s > 1 ? 2.5 : 0.0;
+    const int steps = (ksteps + s - 1) / s;
+    // (tiles in rounds: only whole K is persistent over more tiles than SMs)
+    if (t64 <= most && fixed + slice64 * steps < best) {
+      best = fixed + slice64 * steps;
       split = s;
+      rows64 = true;
+    }
+    if ((t128 <= most || s == 1) &&
+        fixed + slice128 * steps * ((t128 + most - 1) / most) < best) {
+      best = fixed + slice128 * steps * ((t128 + most - 1) / most);
+      split = s;
+      rows64 = false;
     }
   }
-  return launch_form<I8, TA, TB, AT, BT, 64, UNIT, false>(p, split, stream);
+  if (rows64) return launch_form<I8, TA, TB, AT, BT, 64, 64, UNIT, false>(p, split, stream);
+  return launch_form<I8, TA, TB, AT, BT, 128, 64, UNIT, false>(p, split, stream);
 }
 
 inline cudaError_t read_status(int* status, bool clear, cudaStream_t stream) {
