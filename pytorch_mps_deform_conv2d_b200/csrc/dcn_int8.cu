@@ -304,9 +304,11 @@ __device__ __forceinline__ uint64_t raw_pair(const Raw8<T>& r, int j) {
 // (corner offsets, weights with the mask) of all its items in shared memory,
 // neighbouring lanes on neighbouring pixels; then its warps work through the
 // items without waiting for one another, the corners of one vector on their
-// way while the last one's are used.  Bound by the L2 -> SM traffic of the
-// corners (four of 16 bytes for eight codes): the neck's columns in 77 us, 7.3
-// TB/s of corners (100 us with the plans made item by item).
+// way while the last one's are used.  The neck's columns take 80 us (100 with
+// the plans made item by item): 7 TB/s of corners (four of 16 bytes for eight
+// codes), 45% of them from L1.  Bound by the instructions of four warps a
+// scheduler: more corners on their way, with the samples in shared memory
+// instead of registers, took 95 us, more warps with fewer vectors each 89.
 struct alignas(16) PlanI8 {
   int at[4];  // element offsets of the corners within the image
   float w[4];
@@ -361,98 +363,98 @@ sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ o
   int turn = 0;
 #pragma unroll 1
   for (int it = slot; it < mine; it += slots, turn ^= 1) {
-  const long long item = first + it;
-  const int gi = (int)(item / np), lp = (int)(item - (long long)gi * np);
-  const int n = (int)((p0 + lp) / g.P), dg0 = gi * g.Cg / g.cpg;
-  const long long img = (long long)n * g.HW * g.C;
-  uint64_t v[NV][4];  // pairs of fp32
-  float top = 0.f;    // NaN stays
-  // (tap, vector of the tap) of the lane's next vector, and their step
-  const int start = part * 32 + lane, stride = 32 * wpp;
-  int k = start / cvec, cv = start - k * cvec;
-  const int dk = stride / cvec, dc = stride - dk * cvec;
-  // the next vector's corners are on their way while the last one's are used
-  Raw8<T> raw[2][4];
-  float w[2][4];
-  auto fetch = [&](int i) {
-    const bool any = start + i * stride < nvec;
-    const int ch = gi * g.Cg + cv * 8;
-    const PlanI8 q = plans[(any ? k * gdg + (gdg > 1 ? ch / g.cpg - dg0 : 0) : 0) * ib + it];
+    const long long item = first + it;
+    const int gi = (int)(item / np), lp = (int)(item - (long long)gi * np);
+    const int n = (int)((p0 + lp) / g.P), dg0 = gi * g.Cg / g.cpg;
+    const long long img = (long long)n * g.HW * g.C;
+    uint64_t v[NV][4];  // pairs of fp32
+    float top = 0.f;    // NaN stays
+    // (tap, vector of the tap) of the lane's next vector, and their step
+    const int start = part * 32 + lane, stride = 32 * wpp;
+    int k = start / cvec, cv = start - k * cvec;
+    const int dk = stride / cvec, dc = stride - dk * cvec;
+    // the next vector's corners are on their way while the last one's are used
+    Raw8<T> raw[2][4];
+    float w[2][4];
+    auto fetch = [&](int i) {
+      const bool any = start + i * stride < nvec;
+      const int ch = gi * g.Cg + cv * 8;
+      const PlanI8 q = plans[(any ? k * gdg + (gdg > 1 ? ch / g.cpg - dg0 : 0) : 0) * ib + it];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      raw[i & 1][c] = ld8_if<T>(x, img + q.at[c] + ch, any && q.at[c] >= 0);
-      w[i & 1][c] = q.w[c];
-    }
-    k += dk;
-    cv += dc;
-    if (cv >= cvec) {
-      cv -= cvec;
-      ++k;
-    }
-  };
-  fetch(0);
+      for (int c = 0; c < 4; ++c) {
+        raw[i & 1][c] = ld8_if<T>(x, img + q.at[c] + ch, any && q.at[c] >= 0);
+        w[i & 1][c] = q.w[c];
+      }
+      k += dk;
+      cv += dc;
+      if (cv >= cvec) {
+        cv -= cvec;
+        ++k;
+      }
+    };
+    fetch(0);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (i + 1 < NV) fetch(i + 1);
+    for (int i = 0; i < NV; ++i) {
+      if (i + 1 < NV) fetch(i + 1);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[i][j] = 0;
+      for (int j = 0; j < 4; ++j) v[i][j] = 0;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const uint64_t w2 = pair(w[i & 1][c], w[i & 1][c]);
+      for (int c = 0; c < 4; ++c) {
+        const uint64_t w2 = pair(w[i & 1][c], w[i & 1][c]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[i][j] = fma2(raw_pair<T>(raw[i & 1][c], j), w2, v[i][j]);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = unpair(v[i][j]);
-      top = max_abs_nan(max_abs_nan(top, f.x), f.y);
-    }
-  }
-  unsigned bits = __reduce_max_sync(0xffffffffu, abs_bits(top));
-  if (wpp > 1) {  // the item's warps agree on its largest value
-    if (lane == 0) red[turn][warp] = bits;
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "r"(32 * wpp) : "memory");
-    for (int o = 0; o < wpp; ++o) bits = max(bits, red[turn][slot * wpp + o]);
-  }
-  const float s = scale_of(bits);
-  const bool ok = usable_scale(s);
-  // one reciprocal for the item: the samples are rounded sums already, so the
-  // codes are within those roundings of the formula's
-  // (a scale whose reciprocal could overflow divides; one that is not usable
-  // gives zeros)
-  const bool fast = ok && s > 1e-35f;
-  const float inv = fast ? 1.f / s : 0.f;
-  signed char* out = col + ((long long)gi * np + lp) * kp;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int idx = part * 32 + lane + i * 32 * wpp;
-    if (idx < nvec) {
-      // v inv + 1.5 * 2^23: rounded to the nearest whole number, its low byte
-      // the code (|v inv| is 127 at most, up to a rounding)
-      uint32_t b[8];
+        for (int j = 0; j < 4; ++j) v[i][j] = fma2(raw_pair<T>(raw[i & 1][c], j), w2, v[i][j]);
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 f = unpair(v[i][j]);
-        b[2 * j] = __float_as_uint(fmaf(f.x, inv, 12582912.f));
-        b[2 * j + 1] = __float_as_uint(fmaf(f.y, inv, 12582912.f));
+        top = max_abs_nan(max_abs_nan(top, f.x), f.y);
       }
-      uint2 c;
-      c.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-      c.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
-      if (!fast) {
-        float u[8];
+    }
+    unsigned bits = __reduce_max_sync(0xffffffffu, abs_bits(top));
+    if (wpp > 1) {  // the item's warps agree on its largest value
+      if (lane == 0) red[turn][warp] = bits;
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "r"(32 * wpp) : "memory");
+      for (int o = 0; o < wpp; ++o) bits = max(bits, red[turn][slot * wpp + o]);
+    }
+    const float s = scale_of(bits);
+    const bool ok = usable_scale(s);
+    // one reciprocal for the item: the samples are rounded sums already, so the
+    // codes are within those roundings of the formula's
+    // (a scale whose reciprocal could overflow divides; one that is not usable
+    // gives zeros)
+    const bool fast = ok && s > 1e-35f;
+    const float inv = fast ? 1.f / s : 0.f;
+    signed char* out = col + ((long long)gi * np + lp) * kp;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int idx = part * 32 + lane + i * 32 * wpp;
+      if (idx < nvec) {
+        // v inv + 1.5 * 2^23: rounded to the nearest whole number, its low byte
+        // the code (|v inv| is 127 at most, up to a rounding)
+        uint32_t b[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float2 f = unpair(v[i][j]);
-          u[2 * j] = f.x;
-          u[2 * j + 1] = f.y;
+          b[2 * j] = __float_as_uint(fmaf(f.x, inv, 12582912.f));
+          b[2 * j + 1] = __float_as_uint(fmaf(f.y, inv, 12582912.f));
         }
-        c = codes8(u, s, ok);
+        uint2 c;
+        c.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+        c.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
+        if (!fast) {
+          float u[8];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = unpair(v[i][j]);
+            u[2 * j] = f.x;
+            u[2 * j + 1] = f.y;
+          }
+          c = codes8(u, s, ok);
+        }
+        *reinterpret_cast<uint2*>(out + 8 * idx) = c;
       }
-      *reinterpret_cast<uint2*>(out + 8 * idx) = c;
     }
-  }
-  if (part == 0 && lane == 0) scale[(long long)gi * np + lp] = s;
+    if (part == 0 && lane == 0) scale[(long long)gi * np + lp] = s;
   }
 }
 
