@@ -890,52 +890,65 @@ cudaError_t launch_form(const GemmProblem& p, int split, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kern, amap, bmap, g);
 }
 
-// The tiling, by how many SMs it keeps busy.
+// What a tiling costs, in microseconds: `base` for a launch, `slice` for a K
+// slice (128 bytes of K) of one round of tiles, measured on products of 256 to
+// 8192 rows.
+struct TilingCost {
+  double base, slice;
+};
+enum Operands { kOne, kMixed, kTwo, kTwoFine, kInt8 };
+// 256 x 256 on two SMs, 128 x 128, 128 x 64, 64 x 64.  In units of 32 values
+// (kTwoFine) a pair's accumulators wait for drains on the other SM: 2.4 us a
+// slice against 0.81 of its products, so that 128 x 128 wins at every size and
+// pairs are not built for them.
+constexpr TilingCost kTilingCost[5][4] = {
+    {{6.0, 0.60}, {4.2, 0.50}, {3.5, 0.375}, {3.2, 0.27}},
+    {{6.0, 0.90}, {4.2, 0.68}, {3.5, 0.50}, {3.2, 0.34}},
+    {{6.0, 1.24}, {4.2, 0.83}, {3.5, 0.60}, {3.2, 0.42}},
+    {{1e9, 2.40}, {4.2, 1.02}, {3.5, 0.74}, {3.2, 0.60}},
+    {{6.0, 0.38}, {4.2, 0.42}, {3.5, 0.33}, {3.2, 0.27}},
+};
+// K over a cluster divides the slices of the small tilings and costs its
+// barriers and the partial sums' way; of clusters of 4 and 8 no more than 32
+// and 14 fit the SMs' groups at a time.
+constexpr double kClusterCost = 2.5;
+
 template <bool I8, int TA, int TB, bool AT, bool BT, int UNIT>
 cudaError_t launch_tiling(const GemmProblem& p, cudaStream_t stream) {
+  constexpr int KIND = I8 ? kInt8 : TA + TB == 2 ? kOne : TA + TB == 3 ? kMixed
+                       : UNIT == 2 ? kTwoFine : kTwo;
   const long long sms = device_sm_count();
-  auto tiles = [&](int tm, int tn) {
-    return (long long)((p.M + tm - 1) / tm) * ((p.N + tn - 1) / tn) * p.batch;
-  };
-  if (tiles(256, 256) * 2 >= sms) {
-    if constexpr (UNIT == 16 && TA + TB < 4)
-      if (p.coarse) return launch_form<I8, TA, TB, AT, BT, 128, 256, 64, true>(p, 1, stream);
-    return launch_form<I8, TA, TB, AT, BT, 128, 256, UNIT, true>(p, 1, stream);
-  }
-  if (tiles(128, 128) >= sms)
-    return launch_form<I8, TA, TB, AT, BT, 128, 128, UNIT, false>(p, 1, stream);
   const int ksteps = (p.K + (I8 ? 127 : 63)) / (I8 ? 128 : 64);
-  // Small products: the time of one CTA, K slices one after another (measured:
-  // one-term operands 0.26 us a slice in tiles of 64 x 64, 0.28 of 128 x 64;
-  // two-term ones 0.40 and 0.50, to fp32's accuracy 0.59 and 0.68).  K over a
-  // cluster divides the slices and costs 2.5 us (its barriers, the partial
-  // sums' way); of clusters of 4 and 8 no more than 32 and 14 fit the SMs'
-  // groups at a time.
-  const double slice64 = TA + TB == 2 ? 0.26 : UNIT == 2 ? 0.59 : 0.40;
-  const double slice128 = TA + TB == 2 ? 0.28 : UNIT == 2 ? 0.68 : 0.50;
-  const long long t64 = tiles(64, 64), t128 = tiles(128, 64);
+  const int tm[4] = {256, 128, 128, 64}, tn[4] = {256, 128, 64, 64};
   double best = 1e30;
-  int split = 1;
-  bool rows64 = false;
-  for (int s = 1; s <= 8 && s <= ksteps; s *= 2) {
-    const long long most = s == 1 ? sms : s == 2 ? sms / 2 : s == 4 ? 32 : 14;
-    const double fixed = s > 1 ? 2.5 : 0.0;
-    const int steps = (ksteps + s - 1) / s;
-    // (tiles in rounds: only whole K is persistent over more tiles than SMs)
-    if (t64 <= most && fixed + slice64 * steps < best) {
-      best = fixed + slice64 * steps;
-      split = s;
-      rows64 = true;
-    }
-    if ((t128 <= most || s == 1) &&
-        fixed + slice128 * steps * ((t128 + most - 1) / most) < best) {
-      best = fixed + slice128 * steps * ((t128 + most - 1) / most);
-      split = s;
-      rows64 = false;
+  int form = 0, split = 1;
+  for (int f = 0; f < 4; ++f) {
+    const long long mt = (p.M + tm[f] - 1) / tm[f], nt = (p.N + tn[f] - 1) / tn[f];
+    const long long tiles = (p.sym && f < 2 ? mt * (mt + 1) / 2 : mt * nt) * p.batch;
+    const TilingCost c = kTilingCost[KIND][f];
+    for (int s = 1; s <= (f < 2 ? 1 : 8) && s <= ksteps; s *= 2) {
+      const long long slots = f == 0 ? sms / 2 : s == 1 ? sms : s == 2 ? sms / 2
+                              : s == 4 ? 32 : 14;
+      if (s > 1 && tiles > slots) continue;  // a cluster has one tile
+      const double rounds = (double)((tiles + slots - 1) / slots);
+      const double cost = c.base + (s > 1 ? kClusterCost : 0.0) +
+                          rounds * c.slice * ((ksteps + s - 1) / s);
+      if (cost < best) {
+        best = cost;
+        form = f;
+        split = s;
+      }
     }
   }
-  if (rows64) return launch_form<I8, TA, TB, AT, BT, 64, 64, UNIT, false>(p, split, stream);
-  return launch_form<I8, TA, TB, AT, BT, 128, 64, UNIT, false>(p, split, stream);
+  if (form == 3) return launch_form<I8, TA, TB, AT, BT, 64, 64, UNIT, false>(p, split, stream);
+  if (form == 2) return launch_form<I8, TA, TB, AT, BT, 128, 64, UNIT, false>(p, split, stream);
+  if constexpr (KIND != kTwoFine) {
+    if constexpr (!I8 && TA + TB < 4)
+      if (form == 0 && p.coarse)
+        return launch_form<I8, TA, TB, AT, BT, 128, 256, 64, true>(p, 1, stream);
+    if (form == 0) return launch_form<I8, TA, TB, AT, BT, 128, 256, UNIT, true>(p, 1, stream);
+  }
+  return launch_form<I8, TA, TB, AT, BT, 128, 128, UNIT, false>(p, 1, stream);
 }
 
 inline cudaError_t read_status(int* status, bool clear, cudaStream_t stream) {
