@@ -694,7 +694,8 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
         }
         release(&acc_empty[buf]);
       } else {
-        const float f = g.e.factor * (g.e.scale != nullptr ? __ldg(g.e.scale + T.b) : 1.f);
+        // written by a kernel of the same chain of launches: past L1
+        const float f = g.e.factor * (g.e.scale != nullptr ? __ldcg(g.e.scale + T.b) : 1.f);
         uint64_t acc[COLS / 2];
 #pragma unroll
         for (int c = 0; c < COLS / 2; ++c) acc[c] = 0;
@@ -790,7 +791,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
 #pragma unroll
               for (int j = 0; j < 8; ++j) v[j] += w[j];
             }
-            const float f = g.e.factor * (g.e.scale != nullptr ? __ldg(g.e.scale + T.b) : 1.f);
+            const float f = g.e.factor * (g.e.scale != nullptr ? __ldcg(g.e.scale + T.b) : 1.f);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] *= f;
           }

@@ -263,48 +263,65 @@ __device__ __forceinline__ float max_abs_nan(float top, float v) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(v)));
   return r;
 }
-// Eight values as they lie in memory (zeros when not wanted), and the j-th pair
-// of them as fp32.
-template <int T>
-struct Raw8 {
-  uint4 w[T == kF32 ? 2 : 1];
+// VEC values as they lie in memory (zeros when not wanted), and the j-th pair of
+// them as fp32.
+template <int T, int VEC>
+struct Raw {
+  static constexpr int WORDS = VEC * (T == kF32 ? 4 : 2) / 4;
+  uint32_t w[WORDS];
 };
-template <int T>
-__device__ __forceinline__ Raw8<T> ld8_if(const void* p, long long i, bool want) {
-  Raw8<T> r;
-  constexpr int N = T == kF32 ? 2 : 1;
-  const uint4* q = reinterpret_cast<const uint4*>(static_cast<const char*>(p) +
-                                                  i * (T == kF32 ? 4 : 2));
+template <int T, int VEC>
+__device__ __forceinline__ Raw<T, VEC> ld_if(const void* p, long long i, bool want) {
+  Raw<T, VEC> r;
+  constexpr int N = Raw<T, VEC>::WORDS;
+  const uint32_t* q = reinterpret_cast<const uint32_t*>(static_cast<const char*>(p) +
+                                                        i * (T == kF32 ? 4 : 2));
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    r.w[k] = make_uint4(0, 0, 0, 0);
-    if (want) r.w[k] = __ldg(q + k);
+  for (int k = 0; k < N; ++k) r.w[k] = 0;
+  if constexpr (N >= 4) {
+#pragma unroll
+    for (int k = 0; k < N; k += 4) {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (want) u = __ldg(reinterpret_cast<const uint4*>(q + k));
+      r.w[k] = u.x, r.w[k + 1] = u.y, r.w[k + 2] = u.z, r.w[k + 3] = u.w;
+    }
+  } else if constexpr (N == 2) {
+    uint2 u = make_uint2(0, 0);
+    if (want) u = __ldg(reinterpret_cast<const uint2*>(q));
+    r.w[0] = u.x, r.w[1] = u.y;
+  } else {
+    if (want) r.w[0] = __ldg(q);
   }
   return r;
 }
-template <int T>
-__device__ __forceinline__ uint64_t raw_pair(const Raw8<T>& r, int j) {
+template <int T, int VEC>
+__device__ __forceinline__ uint64_t raw_pair(const Raw<T, VEC>& r, int j) {
   if constexpr (T == kF32) {
-    const uint4 u = r.w[j >> 1];
-    return j & 1 ? pair(__uint_as_float(u.z), __uint_as_float(u.w))
-                 : pair(__uint_as_float(u.x), __uint_as_float(u.y));
+    return pair(__uint_as_float(r.w[2 * j]), __uint_as_float(r.w[2 * j + 1]));
   } else {
-    const uint32_t w = j == 0 ? r.w[0].x : j == 1 ? r.w[0].y : j == 2 ? r.w[0].z : r.w[0].w;
+    const uint32_t w = r.w[j];
     if constexpr (T == kBF16T)
       return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
     return pair(f.x, f.y);
   }
 }
+// The low bytes of two words, and of four.
+__device__ __forceinline__ uint32_t low2(uint32_t a, uint32_t b) {
+  return __byte_perm(a, b, 0x0040);
+}
+__device__ __forceinline__ uint32_t low4(const uint32_t* b) {
+  return __byte_perm(low2(b[0], b[1]), low2(b[2], b[3]), 0x5410);
+}
 
-// Channels in eights (per group, per deformable group).  WPP warps share an
-// item (a pixel and group), so that each lane holds at most NV vectors of eight
-// samples in registers from the gather to their codes: the input is gathered
-// once and only codes are written.  A block first makes the sampling plans
-// (corner offsets, weights with the mask) of all its items in shared memory,
-// neighbouring lanes on neighbouring pixels; then its warps work through the
-// items without waiting for one another, the corners of one vector on their
-// way while the last one's are used.  The neck's columns take 80 us (100 with
+// Channels in vectors of VEC (eight, four or two: as groups and deformable
+// groups divide).  WPP warps share an item (a pixel and group), so that each
+// lane holds at most NV vectors of samples in registers from the gather to
+// their codes: the input is gathered once and only codes are written.  A block
+// first makes the sampling plans (corner offsets, weights with the mask) of all
+// its items in shared memory, neighbouring lanes on neighbouring pixels; then
+// its warps work through the items without waiting for one another, the corners
+// of one vector on their way while the last one's are used.  The neck's columns take 80 us (100 with
 // the plans made item by item): 7 TB/s of corners (four of 16 bytes for eight
 // codes), 45% of them from L1.  Bound by the instructions of four warps a
 // scheduler: more corners on their way, with the samples in shared memory
@@ -314,12 +331,12 @@ struct alignas(16) PlanI8 {
   float w[4];
 };
 
-template <int T, int NV>
-__global__ void __launch_bounds__(256, NV > 5 ? 2 : 3)
-sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ off,
-                  const void* __restrict__ mask, long long p0, int np,
-                  signed char* __restrict__ col, int kp, float* __restrict__ scale, int wpp,
-                  int gdg, int ib) {
+template <int T, int VEC, int NV>
+__global__ void __launch_bounds__(256, NV > 5 && VEC == 8 ? 2 : 3)
+sample_vec_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ off,
+                     const void* __restrict__ mask, long long p0, int np,
+                     signed char* __restrict__ col, int kp, float* __restrict__ scale, int wpp,
+                     int gdg, int ib) {
   extern __shared__ PlanI8 plans[];  // [npl][ib]
   __shared__ unsigned red[2][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -359,7 +376,8 @@ sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ o
     plans[i] = q;
   }
   __syncthreads();
-  const int cvec = g.Cg / 8, nvec = g.kk * cvec;
+  constexpr int PAIRS = VEC / 2;
+  const int cvec = g.Cg / VEC, nvec = g.kk * cvec;
   int turn = 0;
 #pragma unroll 1
   for (int it = slot; it < mine; it += slots, turn ^= 1) {
@@ -367,22 +385,22 @@ sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ o
     const int gi = (int)(item / np), lp = (int)(item - (long long)gi * np);
     const int n = (int)((p0 + lp) / g.P), dg0 = gi * g.Cg / g.cpg;
     const long long img = (long long)n * g.HW * g.C;
-    uint64_t v[NV][4];  // pairs of fp32
-    float top = 0.f;    // NaN stays
+    uint64_t v[NV][PAIRS];  // of fp32
+    float top = 0.f;        // NaN stays
     // (tap, vector of the tap) of the lane's next vector, and their step
     const int start = part * 32 + lane, stride = 32 * wpp;
     int k = start / cvec, cv = start - k * cvec;
     const int dk = stride / cvec, dc = stride - dk * cvec;
     // the next vector's corners are on their way while the last one's are used
-    Raw8<T> raw[2][4];
+    Raw<T, VEC> raw[2][4];
     float w[2][4];
     auto fetch = [&](int i) {
       const bool any = start + i * stride < nvec;
-      const int ch = gi * g.Cg + cv * 8;
+      const int ch = gi * g.Cg + cv * VEC;
       const PlanI8 q = plans[(any ? k * gdg + (gdg > 1 ? ch / g.cpg - dg0 : 0) : 0) * ib + it];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        raw[i & 1][c] = ld8_if<T>(x, img + q.at[c] + ch, any && q.at[c] >= 0);
+        raw[i & 1][c] = ld_if<T, VEC>(x, img + q.at[c] + ch, any && q.at[c] >= 0);
         w[i & 1][c] = q.w[c];
       }
       k += dk;
@@ -397,15 +415,16 @@ sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ o
     for (int i = 0; i < NV; ++i) {
       if (i + 1 < NV) fetch(i + 1);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[i][j] = 0;
+      for (int j = 0; j < PAIRS; ++j) v[i][j] = 0;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const uint64_t w2 = pair(w[i & 1][c], w[i & 1][c]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[i][j] = fma2(raw_pair<T>(raw[i & 1][c], j), w2, v[i][j]);
+        for (int j = 0; j < PAIRS; ++j)
+          v[i][j] = fma2(raw_pair<T, VEC>(raw[i & 1][c], j), w2, v[i][j]);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < PAIRS; ++j) {
         const float2 f = unpair(v[i][j]);
         top = max_abs_nan(max_abs_nan(top, f.x), f.y);
       }
@@ -431,37 +450,41 @@ sample8_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict__ o
       if (idx < nvec) {
         // v inv + 1.5 * 2^23: rounded to the nearest whole number, its low byte
         // the code (|v inv| is 127 at most, up to a rounding)
-        uint32_t b[8];
+        uint32_t b[VEC];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < PAIRS; ++j) {
           const float2 f = unpair(v[i][j]);
           b[2 * j] = __float_as_uint(fmaf(f.x, inv, 12582912.f));
           b[2 * j + 1] = __float_as_uint(fmaf(f.y, inv, 12582912.f));
         }
-        uint2 c;
-        c.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-        c.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
         if (!fast) {
-          float u[8];
+          float u[VEC];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < PAIRS; ++j) {
             const float2 f = unpair(v[i][j]);
             u[2 * j] = f.x;
             u[2 * j + 1] = f.y;
           }
-          c = codes8(u, s, ok);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) b[j] = (uint32_t)code_of(u[j], s, ok);
         }
-        *reinterpret_cast<uint2*>(out + 8 * idx) = c;
+        signed char* o = out + VEC * idx;
+        if constexpr (VEC == 8)
+          *reinterpret_cast<uint2*>(o) = make_uint2(low4(b), low4(b + 4));
+        else if constexpr (VEC == 4)
+          *reinterpret_cast<uint32_t*>(o) = low4(b);
+        else
+          *reinterpret_cast<unsigned short*>(o) = (unsigned short)low2(b[0], b[1]);
       }
     }
     if (part == 0 && lane == 0) scale[(long long)gi * np + lp] = s;
   }
 }
 
-template <int T, int NV>
-cudaError_t sample8_form(const Geom& g, const void* x, const void* off, const void* mask,
-                         long long p0, int np, signed char* col, int kp, float* scale, int wpp,
-                         int gdg, cudaStream_t stream) {
+template <int T, int VEC, int NV>
+cudaError_t sample_vec_form(const Geom& g, const void* x, const void* off, const void* mask,
+                            long long p0, int np, signed char* col, int kp, float* scale,
+                            int wpp, int gdg, cudaStream_t stream) {
   const long long items = (long long)np * g.G;
   const int slots = 8 / wpp;
   // items a block: 32, fewer where their plans would take more than 32 KB or
@@ -471,7 +494,7 @@ cudaError_t sample8_form(const Geom& g, const void* x, const void* off, const vo
   while (ib > slots && (ib * one > 32 * 1024 || items < (long long)ib * 3 * device_sm_count()))
     ib /= 2;
   const int smem = one * ib;
-  auto kern = sample8_i8_kernel<T, NV>;
+  auto kern = sample_vec_i8_kernel<T, VEC, NV>;
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
   kern<<<(unsigned)((items + ib - 1) / ib), 256, smem, stream>>>(
@@ -503,14 +526,14 @@ few_tokens_kernel(const void* __restrict__ x, const float* __restrict__ x_scale,
   // the first 8 * 256 * KEEP values of each token are asked for before the
   // weight is, or they would wait for it
   constexpr int KEEP = T == 3 || NT > 2 ? 0 : 2 / NT;
-  Raw8<T == 3 ? 0 : T> raw[NT][KEEP > 0 ? KEEP : 1];
+  Raw<T == 3 ? 0 : T, 8> raw[NT][KEEP > 0 ? KEEP : 1];
   if constexpr (KEEP > 0) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int k = 0; k < KEEP; ++k)
-        raw[t][k] = ld8_if<T>(x, (long long)t * K + 8LL * (tid + 256 * k),
-                              t < tokens && tid + 256 * k < K / 8);
+        raw[t][k] = ld_if<T, 8>(x, (long long)t * K + 8LL * (tid + 256 * k),
+                                t < tokens && tid + 256 * k < K / 8);
   }
   uint4 wv[ROWS][AHEAD];
   const uint4* wr[ROWS];
@@ -533,7 +556,7 @@ few_tokens_kernel(const void* __restrict__ x, const float* __restrict__ x_scale,
     auto kept = [&](int t, int k, float(&v)[8]) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 f = unpair(raw_pair<T>(raw[t][k], j));
+        const float2 f = unpair(raw_pair<T, 8>(raw[t][k], j));
         v[2 * j] = f.x;
         v[2 * j + 1] = f.y;
       }
@@ -662,37 +685,48 @@ cudaError_t few_type(const void* x, const float* x_scale, int tokens, int K, int
   return form(x, x_scale, tokens, K, N, w, w_scale, bias, bias_type, out, out_type, stream);
 }
 
+// Runs the vector kernel where VEC channels divide each group and deformable
+// group (one within the other), and registers and plans hold the items.
+template <int T, int VEC>
+bool sample_vec(const Geom& g, const void* x, const void* off, const void* mask, long long p0,
+                int np, signed char* col, int kp, float* scale, cudaStream_t stream,
+                cudaError_t& e) {
+  const int gdg = g.Cg >= g.cpg ? g.Cg / g.cpg : 1;
+  const bool nested = g.Cg % g.cpg == 0 || g.cpg % g.Cg == 0;
+  const long long nvec = (long long)g.kk * g.Cg / VEC;
+  if (g.Cg % VEC != 0 || g.cpg % VEC != 0 || !nested || nvec > 5 * 32 * 8 ||
+      (reinterpret_cast<uintptr_t>(x) & 15) != 0 ||
+      sizeof(PlanI8) * g.kk * gdg * 8 > 96 * 1024)
+    return false;
+  // one warp an item up to nine vectors a lane (no warp waits for another:
+  // neck 89 -> 81 us), else several with five at most (three blocks an SM
+  // instead of two: the 512-channel sweep 95 us against 99)
+  int wpp = 1;
+  if (nvec > 9 * 32)
+    while (nvec > 5LL * 32 * wpp) wpp *= 2;
+  const long long nv = (nvec + 32 * wpp - 1) / (32 * wpp);
+  auto form = nv <= 1 ? sample_vec_form<T, VEC, 1> : nv <= 3 ? sample_vec_form<T, VEC, 3>
+              : nv <= 5 ? sample_vec_form<T, VEC, 5> : sample_vec_form<T, VEC, 9>;
+  e = form(g, x, off, mask, p0, np, col, kp, scale, wpp, gdg, stream);
+  return true;
+}
+
 template <int T>
 cudaError_t sample_type(const Geom& g, const void* x, const void* off, const void* mask,
                         long long p0, int np, signed char* col, int kp, float* scale,
                         cudaStream_t stream) {
   const long long items = (long long)np * g.G;
-  // eights of channels within each group and deformable group, plans and
-  // registers that hold an item: the vector kernel
-  const int gdg = g.Cg >= g.cpg ? g.Cg / g.cpg : 1;
-  const bool nested = g.Cg % g.cpg == 0 || g.cpg % g.Cg == 0;
-  const long long nvec = (long long)g.kk * g.Cg / 8;
-  if (g.Cg % 8 == 0 && g.cpg % 8 == 0 && nested && nvec <= 5 * 32 * 8 &&
-      (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
-      sizeof(PlanI8) * g.kk * gdg * 8 <= 96 * 1024) {
-    // one warp an item up to nine vectors a lane (no warp waits for another:
-    // neck 89 -> 81 us), else several with five at most (three blocks an SM
-    // instead of two: the 512-channel sweep 95 us against 99)
-    int wpp = 1;
-    if (nvec > 9 * 32)
-      while (nvec > 5LL * 32 * wpp) wpp *= 2;
-    const long long nv = (nvec + 32 * wpp - 1) / (32 * wpp);
-    auto form = nv <= 1 ? sample8_form<T, 1> : nv <= 3 ? sample8_form<T, 3>
-                : nv <= 5 ? sample8_form<T, 5> : sample8_form<T, 9>;
-    return form(g, x, off, mask, p0, np, col, kp, scale, wpp, gdg, stream);
-  }
+  cudaError_t e = cudaSuccess;
+  if (sample_vec<T, 8>(g, x, off, mask, p0, np, col, kp, scale, stream, e)) return e;
+  if (sample_vec<T, 4>(g, x, off, mask, p0, np, col, kp, scale, stream, e)) return e;
+  if (sample_vec<T, 2>(g, x, off, mask, p0, np, col, kp, scale, stream, e)) return e;
   const size_t one = (size_t)g.kk * g.Cg * sizeof(float);
   if (one <= 200 * 1024) {
     int warps = 8;
     while (warps > 1 && one * warps > 100 * 1024) warps >>= 1;
     auto kern = sample_i8_kernel<T, true>;
     const size_t smem = one * warps;
-    cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), (int)smem);
+    e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), (int)smem);
     if (e != cudaSuccess) return e;
     kern<<<(unsigned)((items + warps - 1) / warps), warps * 32, smem, stream>>>(
         g, x, off, mask, p0, np, col, kp, scale);

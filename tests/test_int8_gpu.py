@@ -200,7 +200,10 @@ def ref_deform(k):
     dict(groups=2, dg=4, c=16, o=6), dict(groups=4, dg=2, c=24, o=8), dict(groups=16, c=16, o=16),
     dict(groups=3, dg=3, c=9, o=6), dict(c=1, o=1, n=1, h=1, w=1), dict(c=5, o=300, h=14, w=15),
     dict(n=5, c=20, h=31, w=7, o=130, spread=30.0), dict(c=96, dg=3, groups=2, o=10),
-    dict(c=520, o=16, n=1, h=6, w=5), dict(c=8, o=9, spread=0.0)], ids=str)
+    dict(c=520, o=16, n=1, h=6, w=5), dict(c=8, o=9, spread=0.0),
+    dict(c=40, dg=2, o=8), dict(c=40, dg=4, o=8), dict(c=24, groups=2, dg=1, o=4),
+    dict(c=200, dg=10, kh=5, kw=5, pad=(2, 2), o=4), dict(c=260, dg=2, o=5),
+    dict(c=1100, dg=4, n=1, h=5, w=6, o=4)], ids=str)
 def test_deform_matches_64_bits(cuda_device, case, dtype):
     k = deform_case(**case, dtype=dtype)
     y = run_deform(k)
