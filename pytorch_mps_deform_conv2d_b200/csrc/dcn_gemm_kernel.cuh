@@ -395,11 +395,11 @@ __device__ __forceinline__ void rows32(const GemmArgs& g, const float (&v)[32], 
   }
 }
 
-// 32 channels of one pixel into NCHW planes: a warp's lanes hold neighbouring
-// pixels.
+// 32 channels of one pixel into NCHW planes: a warp's first `rows` lanes hold
+// neighbouring pixels (m < M).
 template <int T>
 __device__ __forceinline__ void planes32(const GemmArgs& g, const float (&v)[32], int b, int m,
-                                         int n0) {
+                                         int n0, int rows) {
   const GemmEpiArgs& e = g.e;
   if (m >= g.M) return;
   const int pixel = e.m_base + m, img = pixel / e.pixels, px = pixel - img * e.pixels;
@@ -409,11 +409,12 @@ __device__ __forceinline__ void planes32(const GemmArgs& g, const float (&v)[32]
     // trade a value, the even one stores channel c of both pixels, the odd one
     // channel c + 1
     if (e.pixel_pairs) {
+      const unsigned lanes = rows >= 32 ? 0xffffffffu : (1u << rows) - 1;
       const bool odd = pixel & 1;
       unsigned short* out = static_cast<unsigned short*>(e.out) + (odd ? at - 1 + e.pixels : at);
 #pragma unroll
       for (int c = 0; c < 32; c += 2) {
-        const float other = __shfl_xor_sync(__activemask(), odd ? v[c] : v[c + 1], 1);
+        const float other = __shfl_xor_sync(lanes, odd ? v[c] : v[c + 1], 1);
         const uint32_t w = odd ? pack2<T>(other, v[c + 1]) : pack2<T>(v[c], other);
         if (n0 + c + odd < g.N)
           *reinterpret_cast<uint32_t*>(out + (long long)c * e.pixels) = w;
@@ -433,9 +434,9 @@ __device__ __forceinline__ void finish32(const GemmArgs& g, float (&v)[32], cons
   const int type = g.e.out_type;
   if constexpr (I8) {
     if (g.e.mode == kEpiPlanes) {
-      if (type == kF32) planes32<kF32>(g, v, T.b, m, n0);
-      else if (type == kBF16T) planes32<kBF16T>(g, v, T.b, m, n0);
-      else planes32<kF16T>(g, v, T.b, m, n0);
+      if (type == kF32) planes32<kF32>(g, v, T.b, m, n0, rows);
+      else if (type == kBF16T) planes32<kBF16T>(g, v, T.b, m, n0, rows);
+      else planes32<kF16T>(g, v, T.b, m, n0, rows);
       return;
     }
   } else {

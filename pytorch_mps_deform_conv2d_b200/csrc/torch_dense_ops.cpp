@@ -9,6 +9,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <utility>
+#include <vector>
+
 #include "dcn_b200.h"
 
 namespace {
@@ -92,6 +96,7 @@ void muon_update_(at::TensorList params, at::TensorList grads, at::TensorList mo
   if (params.empty()) return;
   const uint32_t flags = resolve_math(math);
   std::vector<at::Tensor> aligned(params.size());  // gradients in their parameter's layout
+  std::vector<std::pair<const char*, const char*>> written;  // dense, so ranges of bytes
   for (size_t i = 0; i < params.size(); ++i) {
     const auto &p = params[i], &g = grads[i], &m = momenta[i];
     TORCH_CHECK(p.device().is_cuda() && p.device() == params[0].device() &&
@@ -113,11 +118,17 @@ void muon_update_(at::TensorList params, at::TensorList grads, at::TensorList mo
     TORCH_CHECK(p.numel() == 0 || (rows_outermost(p) && m.strides() == p.strides()),
                 "muon_update_: params must be dense with dimension 0 outermost, momenta of the "
                 "same strides");
-    for (size_t j = 0; j < i; ++j)
-      TORCH_CHECK(p.numel() == 0 || (p.data_ptr() != params[j].data_ptr() &&
-                                     m.data_ptr() != momenta[j].data_ptr()),
-                  "muon_update_: the same parameter or momentum is given twice");
+    if (p.numel() == 0) continue;
+    const char *pb = static_cast<const char*>(p.data_ptr()),
+               *mb = static_cast<const char*>(m.data_ptr());
+    written.emplace_back(pb, pb + p.nbytes());
+    written.emplace_back(mb, mb + m.nbytes());
   }
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i)
+    TORCH_CHECK(written[i].first >= written[i - 1].second,
+                "muon_update_: params and momenta must not overlap (the same parameter or "
+                "momentum is given twice?)");
   c10::cuda::CUDAGuard guard(params[0].device());
   std::vector<bool> done(params.size(), false);
   const auto stream = at::cuda::getCurrentCUDAStream().stream();

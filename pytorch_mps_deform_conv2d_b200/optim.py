@@ -125,7 +125,7 @@ class Muon(torch.optim.Optimizer):
                 self.param_groups.pop()
                 raise ValueError("Muon takes parameters of two dimensions and more; got shape "
                                  f"{tuple(p.shape)} (leave biases to another optimiser)")
-            if p.shape[0] % group["groups"] != 0:
+            if group["groups"] < 1 or p.shape[0] % group["groups"] != 0:
                 self.param_groups.pop()
                 raise ValueError(f"{p.shape[0]} rows are not divisible by "
                                  f"groups={group['groups']}")

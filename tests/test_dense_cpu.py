@@ -33,6 +33,8 @@ def test_optimizer_arguments():
         dcn.Muon([torch.nn.Parameter(torch.randn(6))])
     with pytest.raises(ValueError, match="divisible"):
         dcn.Muon([dict(params=[w], groups=4)])
+    with pytest.raises(ValueError, match="divisible"):
+        dcn.Muon([w], groups=0)
     opt = dcn.Muon([w])
     assert opt.step() is None  # nothing has a gradient: nothing is called
     with pytest.raises(ValueError, match="adjust"):

@@ -247,6 +247,14 @@ def test_muon_refusals(cuda_device):
         assert torch.equal(ps[0], before)
 
 
+def test_muon_refuses_overlapping_views(cuda_device):
+    whole, state = torch.randn(12, 16, device="cuda"), torch.zeros(2, 8, 16, device="cuda")
+    g = torch.randn(8, 16, device="cuda")
+    with pytest.raises(RuntimeError, match="overlap"):
+        dcn.muon_update_([whole[:8], whole[4:]], [g, g], list(state), lr=0.1)
+    dcn.muon_update_([whole[:4], whole[4:]], [g[:4], g], [state[0, :4], state[1]], lr=0.1)
+
+
 def test_muon_bumps_versions(cuda_device):
     ps, gs, ms = leaves([(8, 16)])
     w = ps[0].requires_grad_()
