@@ -911,8 +911,8 @@ constexpr TilingCost kTilingCost[5][4] = {
     {{6.0, 0.38}, {4.2, 0.42}, {3.5, 0.33}, {3.2, 0.27}},
 };
 // K over a cluster divides the slices of the small tilings and costs its
-// barriers and the partial sums' way; of clusters of 4 and 8 no more than 32
-// and 14 fit the SMs' groups at a time.
+// barriers and the partial sums' way; of clusters of 4 and 8 some 33 and 15 fit
+// the SMs' groups at a time.
 constexpr double kClusterCost = 2.5;
 
 template <bool I8, int TA, int TB, bool AT, bool BT, int UNIT>
@@ -922,6 +922,11 @@ cudaError_t launch_tiling(const GemmProblem& p, cudaStream_t stream) {
   const long long sms = device_sm_count();
   const int ksteps = (p.K + (I8 ? 127 : 63)) / (I8 ? 128 : 64);
   const int tm[4] = {256, 128, 128, 64}, tn[4] = {256, 128, 64, 64};
+  using Small = Form<I8, TA, TB, AT, BT, 64, 64, UNIT, false>;
+  const void* small =
+      reinterpret_cast<const void*>(gemm_tc_kernel<I8, TA, TB, AT, BT, 64, 64, UNIT, false>);
+  const cudaError_t e = ensure_dynamic_smem(small, Small::SMEM);
+  if (e != cudaSuccess) return e;
   double best = 1e30;
   int form = 0, split = 1;
   for (int f = 0; f < 4; ++f) {
@@ -929,8 +934,9 @@ cudaError_t launch_tiling(const GemmProblem& p, cudaStream_t stream) {
     const long long tiles = (p.sym && f < 2 ? mt * (mt + 1) / 2 : mt * nt) * p.batch;
     const TilingCost c = kTilingCost[KIND][f];
     for (int s = 1; s <= (f < 2 ? 1 : 8) && s <= ksteps; s *= 2) {
-      const long long slots = f == 0 ? sms / 2 : s == 1 ? sms : s == 2 ? sms / 2
-                              : s == 4 ? 32 : 14;
+      const long long slots =
+          f == 0 ? sms / 2
+                 : s == 1 ? sms : device_cluster_slots(small, THREADS, Small::SMEM, s);
       if (s > 1 && tiles > slots) continue;  // a cluster has one tile
       const double rounds = (double)((tiles + slots - 1) / slots);
       const double cost = c.base + (s > 1 ? kClusterCost : 0.0) +
