@@ -12,6 +12,7 @@ cudaError_t launch_gemm_f16(const GemmProblem& p, cudaStream_t stream) {
     if (ta == 1 && tb == 2) return launch_tiling<false, 1, 2, false, false, 16>(p, stream);
   }
   if (at && bt && ta == 1 && tb == 1) return launch_tiling<false, 1, 1, true, true, 16>(p, stream);
+  if (!at && bt && ta == 1 && tb == 1) return launch_tiling<false, 1, 1, false, true, 16>(p, stream);
   if (!at && bt && ta == 2 && tb == 1) return launch_tiling<false, 2, 1, false, true, 16>(p, stream);
   return cudaErrorInvalidValue;
 }

@@ -233,7 +233,9 @@ __device__ __forceinline__ void store_f(void* p, long long i, float v) {
 // what was stored.
 __device__ __forceinline__ uint4 linear8(const GemmArgs& g, int term, int b, int m, int n) {
   const GemmEpiArgs& e = g.e;
-  if (e.mode != kEpiPoly || m >= g.M || n >= g.N) return make_uint4(0, 0, 0, 0);
+  // (the linear part has the terms of the result)
+  if (e.mode != kEpiPoly || term >= e.out_terms || m >= g.M || n >= g.N)
+    return make_uint4(0, 0, 0, 0);
   return *reinterpret_cast<const uint4*>(e.lin16 + term * e.term_stride +
                                          (long long)b * e.batch_stride +
                                          (long long)m * e.pitch + n);

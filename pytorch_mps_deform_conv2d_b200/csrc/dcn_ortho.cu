@@ -14,7 +14,7 @@
 // part of it, and every further step of the run multiplies that by a^2 while
 // those values grow.  A run ends before the product of its a^2 passes 150:
 // three steps of the usual 3.4445, two runs for five steps; results of 16 bits
-// do not see the difference.  For fp32 results the first run, where one
+// do not see the difference (squarer matrices: run_length below).  For fp32 results the first run, where one
 // direction can hold nearly all of |X|, ends before 12: two steps; so does
 // every run of more than 256 directions.  Emulated in 64 bits on 64 x 576 with
 // a few strong directions, the relative error is 5e-7 with runs (2, 3) and
@@ -233,21 +233,23 @@ Layout layout_of(const OrthoShape& s, int count) {
 }
 
 int run_length(const OrthoShape& s, int first) {
-  // the steps after the first of a run rest on an S that the run itself made
-  // Nearly square matrices gain nothing from longer runs (X costs no more than
-  // S) and lose launches: 1024 x 1024 float32 251 us in single steps, 294 in
-  // runs of 2 and 3; 1024 x 4096 531 and 413.  But X of one term is rounded
-  // once only, after the run that multiplies its errors.
+  // Matrices near enough to square gain nothing from longer runs (X costs
+  // little more than S) and lose launches: 1024 x 1024 float32 251 us in single
+  // steps, 294 in runs of 2 and 3; 1024 x 4096 531 and 413.  With X of one
+  // term its rounding comes after a run of two, and single steps of one-term
+  // squares follow: 1024 x 2048 bf16 207 us, 254 in runs of 3 and 2; 1024 x
+  // 4096 274 and 293, which no longer pays for the rounding.
   const int m = s.rows < s.cols ? s.rows : s.cols, n = s.rows < s.cols ? s.cols : s.rows;
-  if (m > kChainMax && n < 2 * m && (first > 0 || s.later_terms == 2)) return 1;
-  const bool f32 = s.first_terms == 2 && s.later_terms == 2;
+  const bool square = m > kChainMax && n < (s.later_terms == 1 ? 3LL : 2LL) * m;
+  if (square && (first > 0 || s.later_terms == 2)) return 1;
   // The more directions, and the squarer the matrix, the more of them are still
   // small in the second run.
   // Relative errors with runs (2, 3), (2, 2, 1) and of fp32 products: 300 x 2700
   // 0.85e-6, 1.0e-6, 1.5e-6; 515 x 1153 3.2e-6, 2.0e-6, 2.6e-6; 1400 x 2900
   // 6.7e-6, 2.7e-6, 3.8e-6.
-  const float limit =
-      f32 && (first == 0 || m > 256 || n < 2 * m) ? kShortRunLimit : kRunLimit;
+  const bool f32 = s.first_terms == 2 && s.later_terms == 2;
+  const bool few = f32 ? first == 0 || m > 256 || n < 2LL * m : square;
+  const float limit = few ? kShortRunLimit : kRunLimit;
   float grown = 1.f;
   int k = first;
   while (k + 1 < s.steps) {
@@ -361,8 +363,9 @@ cudaError_t launch_ortho(const OrthoShape& s, const OrthoChunk& c, void* workspa
   scale_scope.done();
   if (e != cudaSuccess) return e;
 
+  int sq_terms = 2;  // of the square matrices
   auto square = [&](const unsigned short* base) {
-    GemmOperand o{base, l.m, l.m, l.spitch, 2, l.sterm, c.count, 2 * l.sterm, false};
+    GemmOperand o{base, l.m, l.m, l.spitch, sq_terms, l.sterm, c.count, 2 * l.sterm, false};
     return o;
   };
   auto product = [&](const char* name, const GemmOperand& a, const GemmOperand& b, int M, int N,
@@ -392,7 +395,7 @@ cudaError_t launch_ortho(const OrthoShape& s, const OrthoChunk& c, void* workspa
     q.mode = kEpiTerms;
     q.factor = factor;
     q.out16 = out;
-    q.out_terms = 2;
+    q.out_terms = sq_terms;
     q.pitch = l.spitch;
     q.term_stride = l.sterm;
     q.batch_stride = 2 * l.sterm;
@@ -403,6 +406,13 @@ cudaError_t launch_ortho(const OrthoShape& s, const OrthoChunk& c, void* workspa
   for (int k = 0; k < s.steps;) {
     const int run = run_length(s, k);
     const bool first = k == 0, last = k + run == s.steps;
+    // Where X keeps 11 bits between runs, so do S and P of a later run of one
+    // step: they meet no direction that is still small but with a factor of at
+    // most a, once a step (longer runs multiply S into itself, and earlier
+    // ones have more steps to come).  1024 x 1024 bf16, relative error before
+    // the result's rounding 0.6e-3 -> 1.1e-3, behind it 1.76e-3 -> 1.96e-3
+    // (1.66e-3 for an exact result); half of the operations of those steps.
+    sq_terms = s.later_terms == 1 && run == 1 && !first ? 1 : 2;
     const GemmOperand X{x[cur], s.rows, s.cols, l.xpitch, terms, l.xterm, c.count,
                         terms * l.xterm, !l.wide};
     const float xs = first ? 1.f : 1.f / later_scale;
