@@ -374,7 +374,8 @@ DCN_API int dcn_quantize_int8(int64_t rows, int64_t cols, int type, const void* 
  * the sum exact.  x is int8 with its scales, or floating (x_scale NULL) and
  * coded as by dcn_quantize_int8 inside the call.  At most 131071 input
  * features.  Rows of a multiple of 16 features at 16-byte aligned addresses
- * are read where they lie; others are copied first. */
+ * are read where they lie; others are copied first.  Up to 8 tokens of such
+ * rows (x and weight aligned) need no workspace: it may be NULL there. */
 DCN_API size_t dcn_int8_linear_workspace_size(int64_t tokens, int64_t in_features,
                                               int64_t out_features, int x_type);
 DCN_API int dcn_int8_linear(int64_t tokens, int64_t in_features, int64_t out_features, int x_type,

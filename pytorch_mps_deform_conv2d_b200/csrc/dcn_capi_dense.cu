@@ -300,10 +300,8 @@ DCN_API int dcn_int8_linear(int64_t tokens, int64_t in_features, int64_t out_fea
             "dcn_int8_linear: x, weight, weight_scale and output must not be NULL; x_scale comes "
             "with int8 x and only then");
   LinearPlan p = linear_plan(tokens, in_features, out_features, x_type);
-  if (workspace == nullptr || workspace_bytes < p.total)
+  if (workspace != nullptr && workspace_bytes < p.total)
     return fail(DCN_ERR_WORKSPACE, "dcn_int8_linear: workspace too small");
-  if (!aligned16(x)) p.pack_x = true;
-  if (!aligned16(weight)) p.pack_w = true;
   if (dcn::few_tokens_fit(tokens, in_features) && aligned16(x) && aligned16(weight)) {
     DCN_CUDA(dcn::launch_few_tokens(x, x_type, x_scale, (int)tokens, (int)in_features,
                                     (int)out_features,
@@ -312,6 +310,10 @@ DCN_API int dcn_int8_linear(int64_t tokens, int64_t in_features, int64_t out_fea
              "few_tokens");
     return DCN_OK;
   }
+  if (workspace == nullptr)
+    return fail(DCN_ERR_WORKSPACE, "dcn_int8_linear: these operands need a workspace");
+  if (!aligned16(x)) p.pack_x = true;
+  if (!aligned16(weight)) p.pack_w = true;
   Carve ws(workspace);
   signed char* xq = ws.take<signed char>(p.x_bytes);
   float* xs = ws.take<float>(p.scale_bytes);

@@ -1,9 +1,10 @@
 // dcn_gemm_kernel.cuh -- batched dense products on tcgen05: the kernel and its
-// launch, instantiated by dcn_gemm_f16.cu and dcn_gemm_i8.cu.
+// launch, instantiated by dcn_gemm.cu (8 bits), dcn_gemm_f16.cu and
+// dcn_gemm_f16x2.cu.
 //
 // D[m, n] = sum_k A[m, k] B[n, k].  A CTA (or a pair of CTAs on two SMs) works
 // through tiles: one warp feeds K slices of 128 bytes to shared memory by TMA,
-// one lane issues the products into tensor-memory accumulators, eight warps
+// one elected lane issues the products into tensor-memory accumulators, eight warps
 // drain them.  So loads, products and the epilogue of different moments run at
 // once.  Three tilings:
 //   pairs    256 x 256 on two SMs (cta_group::2), each holding half of both

@@ -6,6 +6,8 @@
 #include <ATen/ATen.h>
 #include <ATen/Context.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
@@ -46,8 +48,16 @@ std::vector<float> step_coefficients(c10::ArrayRef<double> c, int64_t steps, con
   return v;
 }
 
-at::Tensor scratch(size_t bytes, const at::Tensor& like) {
-  return at::empty({(int64_t)std::max<size_t>(bytes, 1)}, like.options().dtype(at::kByte));
+// Bytes for the current stream of the current device, given back at the end of
+// the call: a later allocation of the same stream may have them, other streams
+// not before.
+c10::DataPtr scratch(size_t bytes) {
+  return c10::cuda::CUDACachingAllocator::get()->allocate(std::max<size_t>(bytes, 1));
+}
+
+// Contiguous, on `like`'s device.
+at::Tensor make(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
 }
 
 at::Tensor newton_schulz(const at::Tensor& update, int64_t steps, at::ArrayRef<double> coefficients,
@@ -60,16 +70,16 @@ at::Tensor newton_schulz(const at::Tensor& update, int64_t steps, at::ArrayRef<d
   const auto coef = step_coefficients(coefficients, steps, "newton_schulz");
   c10::cuda::CUDAGuard guard(update.device());
   auto x = update.contiguous();
-  auto out = at::empty(x.sizes(), x.options());
+  auto out = make(x.sizes(), x.scalar_type(), x);
   if (x.numel() == 0) return out;
   const int64_t rows = x.size(-2), cols = x.size(-1), count = x.numel() / (rows * cols);
   const int type = type_code(x.scalar_type());
   const uint32_t flags = resolve_math(math);
   const size_t bytes =
       dcn_newton_schulz_workspace_size(count, rows, cols, type, (int)steps, flags);
-  auto ws = scratch(bytes, x);
+  auto ws = scratch(bytes);
   check_rc(dcn_newton_schulz(count, rows, cols, type, x.data_ptr(), out.data_ptr(), (int)steps,
-                             coef.data(), (float)eps, flags, ws.data_ptr(), bytes,
+                             coef.data(), (float)eps, flags, ws.get(), bytes,
                              at::cuda::getCurrentCUDAStream().stream()));
   return out;
 }
@@ -160,11 +170,11 @@ void muon_update_(at::TensorList params, at::TensorList grads, at::TensorList mo
                                    : std::sqrt(std::max(1.0, (double)rows / (double)cols));
     const size_t bytes = dcn_muon_update_workspace_size((int64_t)p.size(), rows, cols, type,
                                                         (int)steps, flags);
-    auto ws = scratch(bytes, first);
+    auto ws = scratch(bytes);
     check_rc(dcn_muon_update((int64_t)p.size(), rows, cols, type, p.data(), g.data(), m.data(),
                              (float)lr, (float)momentum, nesterov ? 1 : 0, (float)weight_decay,
                              (float)scale, (int)steps, coef.data(), (float)eps, flags,
-                             ws.data_ptr(), bytes, stream));
+                             ws.get(), bytes, stream));
   }
   for (size_t i = 0; i < params.size(); ++i) {  // written through raw pointers
     params[i].unsafeGetTensorImpl()->bump_version();
@@ -179,11 +189,11 @@ std::tuple<at::Tensor, at::Tensor> quantize_int8(const at::Tensor& x) {
   TORCH_CHECK(x.dim() >= 1, "quantize_int8: x must have at least one dimension");
   c10::cuda::CUDAGuard guard(x.device());
   auto xc = x.contiguous();
-  auto q = at::empty(xc.sizes(), xc.options().dtype(at::kChar));
+  auto q = make(xc.sizes(), at::kChar, xc);
   auto sizes = xc.sizes().slice(0, xc.dim() - 1);
   const int64_t cols = xc.size(-1);
   if (cols == 0) return std::make_tuple(q, at::zeros(sizes, xc.options().dtype(at::kFloat)));
-  auto scale = at::empty(sizes, xc.options().dtype(at::kFloat));
+  auto scale = make(sizes, at::kFloat, xc);
   if (xc.numel() == 0) return std::make_tuple(q, scale);
   check_rc(dcn_quantize_int8(xc.numel() / cols, cols, type_code(xc.scalar_type()), xc.data_ptr(),
                              q.data_ptr<int8_t>(), scale.data_ptr<float>(),
@@ -243,18 +253,26 @@ at::Tensor int8_linear(const at::Tensor& x, const at::Tensor& weight,
   }
   auto sizes = xc.sizes().vec();
   sizes.back() = w.size(0);
-  auto out = at::empty(sizes, xc.options().dtype(odt));
+  auto out = make(sizes, odt, xc);
   if (out.numel() == 0) return out;
   const int64_t in = w.size(1), tokens = xc.numel() / in;
   const int xt = type_code(xc.scalar_type());
   const size_t bytes = dcn_int8_linear_workspace_size(tokens, in, w.size(0), xt);
-  auto ws = scratch(bytes, xc);
-  check_rc(dcn_int8_linear(tokens, in, w.size(0), xt, xc.data_ptr(),
+  auto call = [&](void* ws) {
+    return dcn_int8_linear(tokens, in, w.size(0), xt, xc.data_ptr(),
                            given ? xs.data_ptr<float>() : nullptr, w.data_ptr<int8_t>(),
                            ws_.data_ptr<float>(), b.defined() ? b.data_ptr() : nullptr,
                            b.defined() ? type_code(b.scalar_type()) : 0, out.data_ptr(),
-                           type_code(odt), (uint32_t)flags, ws.data_ptr(), bytes,
-                           at::cuda::getCurrentCUDAStream().stream()));
+                           type_code(odt), (uint32_t)flags, ws, ws != nullptr ? bytes : 0,
+                           at::cuda::getCurrentCUDAStream().stream());
+  };
+  // a few tokens take no workspace where their rows allow it
+  int rc = tokens <= 8 ? call(nullptr) : DCN_ERR_WORKSPACE;
+  if (rc == DCN_ERR_WORKSPACE) {
+    auto ws = scratch(bytes);
+    rc = call(ws.get());
+  }
+  check_rc(rc);
   return out;
 }
 
@@ -323,18 +341,18 @@ at::Tensor deform_conv2d_int8(const at::Tensor& input, const at::Tensor& weight,
   auto w = weight.permute({0, 2, 3, 1}).contiguous();  // no copy for a channels-last weight
   auto off = offset.contiguous();
   auto msk = has_mask ? mask->contiguous() : at::Tensor();
-  auto out = at::empty({s.batch, s.out_channels, oh, ow}, x.options().dtype(odt));
+  auto out = make({s.batch, s.out_channels, oh, ow}, odt, x);
   if (out.numel() == 0) return out;
   const uint32_t fl = (uint32_t)flags | (nhwc ? DCN_INPUT_NHWC : 0u);
   const int type = type_code(dt);
   const size_t bytes = dcn_deform_int8_workspace_size(&s, type, fl);
-  auto ws = scratch(bytes, x);
+  auto ws = scratch(bytes);
   check_rc(dcn_deform_int8(&s, type, x.numel() ? x.data_ptr() : nullptr, w.data_ptr<int8_t>(),
                            wscale.data_ptr<float>(), off.data_ptr(),
                            has_mask ? msk.data_ptr() : nullptr,
                            b.defined() ? b.data_ptr() : nullptr,
                            b.defined() ? type_code(b.scalar_type()) : 0, out.data_ptr(),
-                           type_code(odt), fl, ws.data_ptr(), bytes,
+                           type_code(odt), fl, ws.get(), bytes,
                            at::cuda::getCurrentCUDAStream().stream()));
   return out;
 }

@@ -30,15 +30,17 @@ def _flat_coefficients(coefficients: Coefficients) -> List[float]:
 
 
 def _cuda_only(name: str, op: str, t: Tensor) -> None:
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise NotImplementedError(f"pytorch_mps_deform_conv2d_b200.{op} runs on CUDA (sm_100a) "
                                   f"tensors only; {name} is on {t.device}")
 
 
 def _no_grad_only(op: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{op} has no gradient: call it under torch.no_grad() or on detached "
-                           "tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{op} has no gradient: call it under torch.no_grad() or on "
+                                   "detached tensors")
 
 
 def newton_schulz(update: Tensor, steps: int = 5, coefficients: Coefficients = COEFFICIENTS,
@@ -57,7 +59,7 @@ def newton_schulz(update: Tensor, steps: int = 5, coefficients: Coefficients = C
     """
     _cuda_only("update", "newton_schulz", update)
     _no_grad_only("newton_schulz", update)
-    return _ops().newton_schulz(update, int(steps), _flat_coefficients(coefficients), float(eps),
+    return _ops().newton_schulz.default(update, int(steps), _flat_coefficients(coefficients), float(eps),
                                 _flags(None))
 
 
@@ -83,7 +85,7 @@ def muon_update_(params: Sequence[Tensor], grads: Sequence[Tensor], momenta: Seq
         for t in ts:
             _cuda_only(name, "muon_update_", t)
     with torch.no_grad():
-        _ops().muon_update_(list(params), list(grads), list(momenta), float(lr), float(momentum),
+        _ops().muon_update_.default(list(params), list(grads), list(momenta), float(lr), float(momentum),
                             bool(nesterov), float(weight_decay), int(steps),
                             _flat_coefficients(coefficients), float(eps), adjust == "match_rms",
                             int(groups), _flags(None))

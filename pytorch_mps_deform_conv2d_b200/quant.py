@@ -28,7 +28,7 @@ def quantize_int8(x: Tensor) -> Tuple[Tensor, Tensor]:
     A weight (outC, ...) is quantised as ``quantize_int8(weight.flatten(1))``.
     """
     _cuda_only("x", "quantize_int8", x)
-    return _ops().quantize_int8(x.detach())
+    return _ops().quantize_int8.default(x.detach() if x.requires_grad else x)
 
 
 def int8_linear(x: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor] = None,
@@ -42,12 +42,9 @@ def int8_linear(x: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[
     lie; others, and operands off a 16-byte boundary, are copied first.  At
     most 131071 features.
     """
-    for name, t in (("x", x), ("weight", weight), ("weight_scale", weight_scale),
-                    ("bias", bias), ("x_scale", x_scale)):
-        if t is not None:
-            _cuda_only(name, "int8_linear", t)
+    _cuda_only("x", "int8_linear", x)
     _no_grad_only("int8_linear", x, weight_scale, bias, x_scale)
-    return _ops().int8_linear(x, weight, weight_scale, bias, x_scale, out_dtype)
+    return _ops().int8_linear.default(x, weight, weight_scale, bias, x_scale, out_dtype)
 
 
 def deform_conv2d_int8(input: Tensor, offset: Tensor, weight: Tensor, weight_scale: Tensor,
@@ -65,17 +62,14 @@ def deform_conv2d_int8(input: Tensor, offset: Tensor, weight: Tensor, weight_sca
     ``mask_logits`` as in :func:`deform_conv2d_ex`.
     """
     stride, padding, dilation = _pair(stride), _pair(padding), _pair(dilation)
-    for name, t in (("input", input), ("offset", offset), ("weight", weight),
-                    ("weight_scale", weight_scale), ("bias", bias), ("mask", mask)):
-        if t is not None:
-            _cuda_only(name, "deform_conv2d_int8", t)
+    _cuda_only("input", "deform_conv2d_int8", input)
     _no_grad_only("deform_conv2d_int8", input, offset, weight_scale, bias, mask)
-    if weight.dim() != 4 or weight.shape[1] == 0:
+    shape = weight.shape
+    if len(shape) != 4 or shape[1] == 0:
         raise RuntimeError("weight must be 4-D (outC, C/groups, kh, kw) with C/groups > 0")
-    kh, kw = weight.shape[-2], weight.shape[-1]
-    groups = input.shape[1] // weight.shape[1]
-    deformable_groups = offset.shape[1] // (2 * kh * kw)
-    return _ops().deform_conv2d_int8(
+    groups = input.shape[1] // shape[1]
+    deformable_groups = offset.shape[1] // (2 * shape[2] * shape[3])
+    return _ops().deform_conv2d_int8.default(
         input, weight, weight_scale, offset, mask, bias, stride[0], stride[1], padding[0],
         padding[1], dilation[0], dilation[1], groups, deformable_groups, out_dtype,
         MASK_LOGITS if mask_logits and mask is not None else 0)
@@ -118,10 +112,15 @@ class Int8DeformConv2d(nn.Module):
             self.weight_scale = scale.to(self.weight_scale.device)
         return self
 
-    @torch.no_grad()
     def forward(self, input: Tensor, offset: Optional[Tensor] = None,
                 mask: Optional[Tensor] = None,
                 out_dtype: Optional[torch.dtype] = None) -> Tensor:
+        if torch.is_grad_enabled():
+            with torch.no_grad():
+                return self._forward(input, offset, mask, out_dtype)
+        return self._forward(input, offset, mask, out_dtype)
+
+    def _forward(self, input, offset, mask, out_dtype):
         logits = False
         if self.conv_offset is not None:
             if offset is not None or mask is not None:

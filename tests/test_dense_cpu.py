@@ -99,6 +99,11 @@ def test_int8_c_refusals():
     assert call(o=None) == INVALID and call(ot=I8) == INVALID and call(b=P, bt=I8) == INVALID
     assert call(cin=0) == INVALID and call(cin=131072) == UNSUPPORTED
     assert call(n=ws - 1) == WORKSPACE and call(tokens=0) == OK
+    # without a workspace: only a few tokens, of whole and aligned rows
+    none = lambda tokens, cin, w: lib.dcn_int8_linear(  # noqa: E731
+        tokens, cin, 32, F16, P, None, w, P, None, F32, P, F16, 0, None, 0, None)
+    assert none(9, 64, P) == WORKSPACE and none(4, 63, P) == WORKSPACE
+    assert none(4, 64, P + 1) == WORKSPACE
 
 
 def test_deform_int8_c_refusals():
