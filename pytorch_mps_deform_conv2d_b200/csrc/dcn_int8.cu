@@ -263,34 +263,27 @@ __device__ __forceinline__ float max_abs_nan(float top, float v) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(v)));
   return r;
 }
-// VEC values as they lie in memory (zeros when not wanted), and the j-th pair of
-// them as fp32.
+// VEC values as they lie in memory, and the j-th pair of them as fp32.
 template <int T, int VEC>
 struct Raw {
   static constexpr int WORDS = VEC * (T == kF32 ? 4 : 2) / 4;
   uint32_t w[WORDS];
 };
 template <int T, int VEC>
-__device__ __forceinline__ Raw<T, VEC> ld_if(const void* p, long long i, bool want) {
+__device__ __forceinline__ Raw<T, VEC> ld_raw(const void* p) {
   Raw<T, VEC> r;
   constexpr int N = Raw<T, VEC>::WORDS;
-  const uint32_t* q = reinterpret_cast<const uint32_t*>(static_cast<const char*>(p) +
-                                                        i * (T == kF32 ? 4 : 2));
-#pragma unroll
-  for (int k = 0; k < N; ++k) r.w[k] = 0;
   if constexpr (N >= 4) {
 #pragma unroll
     for (int k = 0; k < N; k += 4) {
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (want) u = __ldg(reinterpret_cast<const uint4*>(q + k));
+      const uint4 u = __ldg(static_cast<const uint4*>(p) + k / 4);
       r.w[k] = u.x, r.w[k + 1] = u.y, r.w[k + 2] = u.z, r.w[k + 3] = u.w;
     }
   } else if constexpr (N == 2) {
-    uint2 u = make_uint2(0, 0);
-    if (want) u = __ldg(reinterpret_cast<const uint2*>(q));
+    const uint2 u = __ldg(static_cast<const uint2*>(p));
     r.w[0] = u.x, r.w[1] = u.y;
   } else {
-    if (want) r.w[0] = __ldg(q);
+    r.w[0] = __ldg(static_cast<const uint32_t*>(p));
   }
   return r;
 }
@@ -327,8 +320,8 @@ __device__ __forceinline__ uint32_t low4(const uint32_t* b) {
 // four warps a scheduler: more corners on their way, with the samples in shared
 // memory instead of registers, took 95 us, more warps with fewer vectors each 89.
 struct alignas(16) PlanI8 {
-  int at[4];  // element offsets of the corners within the image
-  float w[4];
+  int at[4];      // element offsets of the corners within the image
+  uint64_t w[4];  // their weights, twice each: operands of packed multiply-adds
 };
 
 template <int T, int VEC, int NV>
@@ -362,28 +355,36 @@ sample_vec_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict_
       if (g.mask_logits) m = 1.f / (1.f + expf(-m));
     }
     const Sample sp = make_sample(h, w, g.H, g.W);
+    // A dropped corner has weight 0 (whatever the mask is) and reads one that is
+    // not dropped; without any, the first offset is -1 and the sample 0.
+    const int corner[4] = {sp.i1, sp.i2, sp.i3, sp.i4};
+    const float weight[4] = {sp.w1, sp.w2, sp.w3, sp.w4};
+    int some = -1;
+#pragma unroll
+    for (int c = 3; c >= 0; --c)
+      if (sp.live >> c & 1u) some = corner[c] * g.C;
     PlanI8 q;
-    // a dropped corner: offset -1, not read
-    q.at[0] = sp.live & 1u ? sp.i1 * g.C : -1;
-    q.at[1] = sp.live & 2u ? sp.i2 * g.C : -1;
-    q.at[2] = sp.live & 4u ? sp.i3 * g.C : -1;
-    q.at[3] = sp.live & 8u ? sp.i4 * g.C : -1;
-    // (nor weighted: a mask that is not finite must not reach it)
-    q.w[0] = sp.live & 1u ? sp.w1 * m : 0.f;
-    q.w[1] = sp.live & 2u ? sp.w2 * m : 0.f;
-    q.w[2] = sp.live & 4u ? sp.w3 * m : 0.f;
-    q.w[3] = sp.live & 8u ? sp.w4 * m : 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const bool live = sp.live >> c & 1u;
+      const float wc = live ? weight[c] * m : 0.f;
+      q.at[c] = live ? corner[c] * g.C : some;
+      q.w[c] = pair(wc, wc);
+    }
     plans[i] = q;
   }
   __syncthreads();
   constexpr int PAIRS = VEC / 2;
+  constexpr int SIZE = T == kF32 ? 4 : 2;
   const int cvec = g.Cg / VEC, nvec = g.kk * cvec;
+  // vectors of a deformable group, and a reciprocal (exact: products below 2^32)
+  const unsigned cpv = g.cpg / VEC, cpv_inv = 0xffffffffu / cpv + 1;
   int turn = 0;
 #pragma unroll 1
   for (int it = slot; it < mine; it += slots, turn ^= 1) {
     const long long item = first + it;
     const int gi = (int)(item / np), lp = (int)(item - (long long)gi * np);
-    const int n = (int)((p0 + lp) / g.P), dg0 = gi * g.Cg / g.cpg;
+    const int n = (int)((p0 + lp) / g.P);
     const long long img = (long long)n * g.HW * g.C;
     uint64_t v[NV][PAIRS];  // of fp32
     float top = 0.f;        // NaN stays
@@ -393,14 +394,20 @@ sample_vec_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict_
     const int dk = stride / cvec, dc = stride - dk * cvec;
     // the next vector's corners are on their way while the last one's are used
     Raw<T, VEC> raw[2][4];
-    float w[2][4];
+    uint64_t w[2][4];
+    bool live[2];
+    const char* base = static_cast<const char*>(x) + (img + gi * g.Cg) * SIZE;
     auto fetch = [&](int i) {
-      const bool any = start + i * stride < nvec;
-      const int ch = gi * g.Cg + cv * VEC;
-      const PlanI8 q = plans[(any ? k * gdg + (gdg > 1 ? ch / g.cpg - dg0 : 0) : 0) * ib + it];
+      const bool inside = start + i * stride < nvec;
+      const int sub = gdg > 1 ? (cpv == 1 ? cv : (int)__umulhi((unsigned)cv, cpv_inv)) : 0;
+      const PlanI8& q = plans[(inside ? k * gdg + sub : 0) * ib + it];
+      const int4 at = *reinterpret_cast<const int4*>(q.at);
+      live[i & 1] = inside && at.x >= 0;
+      const char* ch = base + cv * (VEC * SIZE);
+      const int o[4] = {at.x, at.y, at.z, at.w};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        raw[i & 1][c] = ld_if<T, VEC>(x, img + q.at[c] + ch, any && q.at[c] >= 0);
+        raw[i & 1][c] = ld_raw<T, VEC>(ch + (long long)max(o[c], 0) * SIZE);
         w[i & 1][c] = q.w[c];
       }
       k += dk;
@@ -417,11 +424,13 @@ sample_vec_i8_kernel(Geom g, const void* __restrict__ x, const void* __restrict_
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) v[i][j] = 0;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint64_t w2 = pair(w[i & 1][c], w[i & 1][c]);
+      for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int j = 0; j < PAIRS; ++j)
-          v[i][j] = fma2(raw_pair<T, VEC>(raw[i & 1][c], j), w2, v[i][j]);
+          v[i][j] = fma2(raw_pair<T, VEC>(raw[i & 1][c], j), w[i & 1][c], v[i][j]);
+      if (!live[i & 1]) {
+#pragma unroll
+        for (int j = 0; j < PAIRS; ++j) v[i][j] = 0;
       }
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) {
@@ -532,8 +541,11 @@ few_tokens_kernel(const void* __restrict__ x, const float* __restrict__ x_scale,
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int k = 0; k < KEEP; ++k)
-        raw[t][k] = ld_if<T, 8>(x, (long long)t * K + 8LL * (tid + 256 * k),
-                                t < tokens && tid + 256 * k < K / 8);
+        if (t < tokens && tid + 256 * k < K / 8)
+          raw[t][k] = ld_raw<T, 8>(static_cast<const char*>(x) +
+                                   ((long long)t * K + 8LL * (tid + 256 * k)) * (T == kF32 ? 4 : 2));
+        else
+          raw[t][k] = {};
   }
   uint4 wv[ROWS][AHEAD];
   const uint4* wr[ROWS];
@@ -694,7 +706,7 @@ bool sample_vec(const Geom& g, const void* x, const void* off, const void* mask,
   const int gdg = g.Cg >= g.cpg ? g.Cg / g.cpg : 1;
   const bool nested = g.Cg % g.cpg == 0 || g.cpg % g.Cg == 0;
   const long long nvec = (long long)g.kk * g.Cg / VEC;
-  if (g.Cg % VEC != 0 || g.cpg % VEC != 0 || !nested || nvec > 5 * 32 * 8 ||
+  if (g.HW == 0 || g.Cg % VEC != 0 || g.cpg % VEC != 0 || !nested || nvec > 5 * 32 * 8 ||
       (reinterpret_cast<uintptr_t>(x) & 15) != 0 ||
       sizeof(PlanI8) * g.kk * gdg * 8 > 96 * 1024)
     return false;
