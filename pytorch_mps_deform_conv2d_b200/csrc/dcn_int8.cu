@@ -315,10 +315,12 @@ __device__ __forceinline__ uint32_t low4(const uint32_t* b) {
 // its items in shared memory, neighbouring lanes on neighbouring pixels; then
 // its warps work through the items without waiting for one another, the corners
 // of one vector on their way while the last one's are used.  The neck's columns
-// take 80 us (100 with the plans made item by item): 7 TB/s of corners (four of
-// 16 bytes for eight codes), 45% of them from L1.  Bound by the instructions of
-// four warps a scheduler: more corners on their way, with the samples in shared
-// memory instead of registers, took 95 us, more warps with fewer vectors each 89.
+// take 75 us (100 with the plans made item by item): 7.5 TB/s of corners (four
+// of 16 bytes for eight codes), 40% of them from L1.  Bound by the instructions
+// and latencies of four warps a scheduler, which issue in 60% of the cycles:
+// more corners on their way, with the samples in shared memory instead of
+// registers, took 95 us, more warps with fewer vectors each 89; a walk through
+// the pixels in tiles of 8 x 4 changed nothing.
 struct alignas(16) PlanI8 {
   int at[4];      // element offsets of the corners within the image
   uint64_t w[4];  // their weights, twice each: operands of packed multiply-adds
