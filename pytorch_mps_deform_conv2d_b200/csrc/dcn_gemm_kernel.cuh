@@ -642,8 +642,13 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
         else tc::mbar_arrive(bar);
       }
     };
-    int n = 0, unit = 0;
-    for (int t = first_tile; t < g.tiles; t += tile_step, ++n) {
+    int unit = 0;
+    // int8: false once a wait of this warp has run out.  Such a warp touches no
+    // accumulator any more, but still meets the other seven at the named barrier
+    // of every tile left: one of them may have found the accumulators complete a
+    // moment later, and that barrier has no limit.
+    bool live = true;
+    for (int t = first_tile; t < g.tiles; t += tile_step) {
       const Tile T = tile_of<F, PAIR>(g, t, rank);
       // (64 rows of A lie in the first 16 lanes of each quarter)
       const int first = T.m0 + q * F::WROWS, rows = min(F::WROWS, g.M - first);
@@ -663,7 +668,9 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
         }
         asm volatile("bar.sync 1, %0;" ::"n"(EPI_WARPS * 32) : "memory");
         const int buf = unit % F::BUFS;
-        if (!tc::wait(watch, &acc_full[buf], (unit / F::BUFS) & 1)) break;
+        // (whole warps: the loads of tensor memory that follow take all lanes)
+        live = live && wait_warp(watch, &acc_full[buf], (unit / F::BUFS) & 1);
+        if (!live) continue;
         ++unit;
         tc::tc_fence_after();
         if (g.split > 1) {
@@ -707,10 +714,8 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
 #pragma unroll 1
         for (int u = 0; u < units; ++u, ++unit) {
           const int buf = unit % F::BUFS;
-          if (!tc::wait(watch, &acc_full[buf], (unit / F::BUFS) & 1)) {
-            ok = false;
-            break;
-          }
+          ok = wait_warp(watch, &acc_full[buf], (unit / F::BUFS) & 1);
+          if (!ok) break;
           tc::tc_fence_after();
 #pragma unroll
           for (int c = 0; c < COLS; c += 32) {

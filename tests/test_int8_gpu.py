@@ -379,3 +379,15 @@ def test_train_with_muon_then_serve_in_8_bits(cuda_device, modulated):
     plain = dcn.Int8DeformConv2d.from_float(dcn.DeformConv2d(8, 8, 3).cuda())
     with pytest.raises(TypeError, match="offset"):
         plain(torch.randn(1, 8, 5, 5, device="cuda"))
+
+
+@pytest.mark.parametrize("tokens,cin,cout", [(4096, 64, 4096), (6000, 640, 3000), (40000, 64, 64)])
+def test_waits_that_run_out_over_many_tiles_are_reported(cuda_device, tokens, cin, cout):
+    # more tiles than CTAs: a CTA that gives up still walks through those it has left
+    dcn.device_status()
+    q, w, s = rand_codes(tokens, cin), rand_codes(cout, cin), torch.rand(cout, device="cuda")
+    xs = torch.rand(tokens, device="cuda")
+    _native.load_ops().int8_linear(q, w, s, None, xs, None, TEST_WAIT_TIMEOUT)
+    assert dcn.device_status() & STATUS_DENSE_TIMEOUT
+    check_linear(dcn.int8_linear(q, w, s, x_scale=xs), q, xs, w, s, None)
+    dcn.check_device_status()

@@ -323,3 +323,13 @@ def test_optimizer_step_in_a_graph(cuda_device):
         graph.replay()
         opts[1].step()
     assert torch.equal(layer.weight, twin.weight)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_waits_that_run_out_over_many_tiles_are_reported(cuda_device, dtype):
+    dcn.device_status()
+    x = gradient(6, 700, 900, dtype=dtype)
+    _native.load_ops().newton_schulz(x, 5, list(COEF), 1e-7, TEST_WAIT_TIMEOUT)
+    assert dcn.device_status() & STATUS_DENSE_TIMEOUT
+    assert rel(dcn.newton_schulz(x), orthogonalise(x)) <= TOL[dtype]
+    dcn.check_device_status()
