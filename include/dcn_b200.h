@@ -334,8 +334,8 @@ DCN_API int dcn_h16_staging(const dcn_shape* shape, uint32_t flags);
  * matrices keep what their type can hold.  A matrix with NaN or an infinity
  * gives NaN everywhere.  Made for polynomials that keep singular values of
  * [0, 1] below 2: S is held up to 8, a I + b S + c S S up to 16; beyond, results
- * may be NaN.  At most 32 steps, coefficients of 15, 2^31 - 1 elements and a
- * smaller side of 32768. */
+ * may be NaN.  At most 32 steps, coefficients of 15, 2^31 - 1 elements, a
+ * larger side of 2^31 - 256 and a smaller one of 32768. */
 DCN_API size_t dcn_newton_schulz_workspace_size(int64_t count, int64_t rows, int64_t cols,
                                                 int type, int steps, uint32_t flags);
 DCN_API int dcn_newton_schulz(int64_t count, int64_t rows, int64_t cols, int type,
@@ -373,7 +373,7 @@ DCN_API int dcn_quantize_int8(int64_t rows, int64_t cols, int type, const void* 
  *   output = (sum_k x weight) x_scale[token] weight_scale[channel] + bias,
  * the sum exact.  x is int8 with its scales, or floating (x_scale NULL) and
  * coded as by dcn_quantize_int8 inside the call.  At most 131071 input
- * features.  Rows of a multiple of 16 features at 16-byte aligned addresses
+ * features, 2^31 - 256 tokens and as many outputs.  Rows of a multiple of 16 features at 16-byte aligned addresses
  * are read where they lie; others are copied first.  Up to 8 tokens of such
  * rows (x and weight aligned) need no workspace: it may be NULL there. */
 DCN_API size_t dcn_int8_linear_workspace_size(int64_t tokens, int64_t in_features,
@@ -391,7 +391,8 @@ DCN_API int dcn_int8_linear(int64_t tokens, int64_t in_features, int64_t out_fea
  * they lie, others are copied first).  The sampled columns of each output pixel and group are
  * coded as by dcn_quantize_int8 (a token), their products with the weight
  * scaled back.  `flags`: DCN_MASK_LOGITS, DCN_INPUT_NHWC.  The output is dense
- * NCHW of `out_type`. */
+ * NCHW of `out_type`.  At most 131071 columns and 2^31 - 256 output channels a
+ * group. */
 DCN_API size_t dcn_deform_int8_workspace_size(const dcn_shape* shape, int type, uint32_t flags);
 DCN_API int dcn_deform_int8(const dcn_shape* shape, int type, const void* input,
                             const int8_t* weight, const float* weight_scale, const void* offset,

@@ -23,6 +23,9 @@ constexpr size_t kOrthoChunkBytes = size_t(1) << 30;
 constexpr size_t kColumnBytes = size_t(256) << 20;
 // |sum| <= K * 128 * 128 stays inside int32
 constexpr int64_t kInt8MaxK = 131071;
+// Rows and columns of a product: the kernels round them up to whole tiles, of
+// 256 at most, in int
+constexpr int64_t kMaxSide = (int64_t(1) << 31) - 256;
 
 int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -60,9 +63,9 @@ int ortho_shape(int64_t rows, int64_t cols, int type, int steps, const float* co
             dcn::kOrthoMaxSteps, steps);
   DCN_CHECK(eps >= 0.f, "%s: eps must be non-negative", op);
   const int64_t small = rows < cols ? rows : cols, large = rows < cols ? cols : rows;
-  if (small > 32768 || large >= (int64_t(1) << 31) || small * large >= (int64_t(1) << 31))
-    return fail(DCN_ERR_UNSUPPORTED, "%s: matrices of 2^31 elements and more, or with both sides "
-                "beyond 32768, are not supported", op);
+  if (small > 32768 || large > kMaxSide || small * large >= (int64_t(1) << 31))
+    return fail(DCN_ERR_UNSUPPORTED, "%s: matrices of 2^31 elements and more, with a side beyond "
+                "2^31 - 256 or with both sides beyond 32768, are not supported", op);
   const uint32_t math = flags & 0xff;
   const bool f32 = type == DCN_TYPE_F32;
   s.rows = (int)rows;
@@ -104,6 +107,9 @@ int deform_int8_plan(const dcn_shape* shape, int type, uint32_t flags, DeformInt
   const dcn::Geom& g = d.g;
   if (!(flags & DCN_INPUT_NHWC) && g.N > 65535)
     return fail(DCN_ERR_UNSUPPORTED, "%s: more than 65535 NCHW images are not supported", op);
+  if (g.Og > kMaxSide)
+    return fail(DCN_ERR_UNSUPPORTED, "%s: more than %lld output channels a group are not supported",
+                op, (long long)kMaxSide);
   d.kg = (int64_t)g.Cg * g.kk;
   if (d.kg > kInt8MaxK)
     return fail(DCN_ERR_UNSUPPORTED, "%s: more than %lld columns a group are not supported", op,
@@ -290,10 +296,10 @@ DCN_API int dcn_int8_linear(int64_t tokens, int64_t in_features, int64_t out_fea
             "dcn_int8_linear: x must be float32, bfloat16, float16 or int8");
   DCN_CHECK(float_type(out_type) && (bias == nullptr || float_type(bias_type)),
             "dcn_int8_linear: output and bias must be float32, bfloat16 or float16");
-  if (in_features > kInt8MaxK || tokens >= (int64_t(1) << 31) - 128 ||
-      out_features >= (int64_t(1) << 31) - 256)
+  if (in_features > kInt8MaxK || tokens > kMaxSide || out_features > kMaxSide)
     return fail(DCN_ERR_UNSUPPORTED, "dcn_int8_linear: more than %lld input features (sums past "
-                "int32) or 2^31 rows are not supported", (long long)kInt8MaxK);
+                "int32), or than %lld tokens or outputs, are not supported", (long long)kInt8MaxK,
+                (long long)kMaxSide);
   if (tokens == 0 || out_features == 0) return DCN_OK;
   DCN_CHECK(x != nullptr && weight != nullptr && weight_scale != nullptr && output != nullptr &&
                 ((x_type == DCN_TYPE_I8) == (x_scale != nullptr)),

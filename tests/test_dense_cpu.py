@@ -152,3 +152,31 @@ def test_operators_infer_shapes():
                                meta(2, 18, 9, 9), None, None, 1, 1, 1, 1, 1, 1, 1, 1,
                                torch.bfloat16)
     assert y.shape == (2, 6, 9, 9) and y.dtype == torch.bfloat16
+
+
+def test_sides_that_tiles_would_round_past_31_bits_are_refused():
+    # the last refused by its workspace: the size itself is taken
+    lib = _native.load_capi()
+    c, top = coef(3.4, -4.8, 2.0), (1 << 31) - 256
+
+    def schulz(rows, cols):
+        return lib.dcn_newton_schulz(1, rows, cols, F32, P, P, 1, c, 0.0, 0, P, 16, None)
+
+    def linear(tokens, cout):
+        return lib.dcn_int8_linear(tokens, 16, cout, I8, P, P, P, P, None, F32, P, F32, 0, P, 16,
+                                   None)
+
+    def deform(cout):
+        s = _native.DcnShape(batch=1, in_channels=1, height=1, width=1, out_channels=cout,
+                             kernel_h=1, kernel_w=1, stride_h=1, stride_w=1, pad_h=0, pad_w=0,
+                             dilation_h=1, dilation_w=1, groups=1, deformable_groups=1)
+        return lib.dcn_deform_int8(ctypes.byref(s), F32, P, P, P, P, None, None, F32, P, F32, 0, P,
+                                   16, None)
+
+    for call in (lambda n: schulz(1, n), lambda n: schulz(n, 1), lambda n: linear(n, 1),
+                 lambda n: linear(1, n), deform):
+        assert call(top + 1) == UNSUPPORTED and call((1 << 31) - 1) == UNSUPPORTED
+        assert call(top) == WORKSPACE
+    for n in (top + 1, (1 << 31) - 1):
+        assert lib.dcn_newton_schulz_workspace_size(1, 1, n, F32, 1, 0) == 0
+        assert lib.dcn_muon_update_workspace_size(1, n, 1, F32, 1, 0) == 0
