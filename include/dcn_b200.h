@@ -331,8 +331,8 @@ DCN_API int dcn_h16_staging(const dcn_shape* shape, uint32_t flags);
  * memory: (a, b, c) of each step.  `output` may be `input`.  The products run
  * on the tensor cores: float32 matrices keep fp32 accuracy (two fp16 terms an
  * operand), or that of one TF32 product with DCN_MATH_TF32 in `flags`; 16-bit
- * matrices keep what their type can hold.  A matrix with NaN or an infinity
- * gives NaN everywhere.  Made for polynomials that keep singular values of
+ * matrices keep what their type can hold.  A matrix of zeros stays zero for any
+ * eps; one with NaN or an infinity gives NaN everywhere.  Made for polynomials that keep singular values of
  * [0, 1] below 2: S is held up to 8, a I + b S + c S S up to 16; beyond, results
  * may be NaN.  At most 32 steps, coefficients of 15, 2^31 - 1 elements, a
  * larger side of 2^31 - 256 and a smaller one of 32768. */

@@ -152,9 +152,11 @@ __global__ void __launch_bounds__(256) ortho_scale_kernel(const __grid_constant_
       f1 = (float)ldexp(1.0, k / 2);
       f2 = (float)ldexp(1.0, k - k / 2);
       if (blockIdx.x == 0) {
-        // a norm that is not finite leaves nothing to scale by
-        const float r = isfinite(norm) ? (float)ldexp(1.0 / (norm + (double)a.eps), -k)
-                                       : __int_as_float(0x7fc00000);
+        // a norm that is not finite leaves nothing to scale by; a matrix of zeros
+        // is its own answer, whatever 1 / eps (squared for the Gram matrix) is
+        const float r = !isfinite(norm) ? __int_as_float(0x7fc00000)
+                        : norm == 0.0   ? 0.f
+                                        : (float)ldexp(1.0 / (norm + (double)a.eps), -k);
         a.r1[b] = r;
         a.r2[b] = r * r;
       }

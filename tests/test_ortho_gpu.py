@@ -333,3 +333,26 @@ def test_waits_that_run_out_over_many_tiles_are_reported(cuda_device, dtype):
     assert dcn.device_status() & STATUS_DENSE_TIMEOUT
     assert rel(dcn.newton_schulz(x), orthogonalise(x)) <= TOL[dtype]
     dcn.check_device_status()
+
+
+@pytest.mark.parametrize("eps", [1e-7, 1e-20, 1e-37, 0.0])
+@pytest.mark.parametrize("shape", [(2, 48, 80), (2, 80, 48), (2, 150, 200), (2, 200, 500)], ids=str)
+def test_zeros_stay_zero_whatever_eps_is(cuda_device, shape, eps):
+    # (1 / eps and its square leave fp32's range)
+    for dtype in DTYPES:
+        x = gradient(*shape, dtype=dtype)
+        x[0] = 0
+        y = dcn.newton_schulz(x, eps=eps)
+        assert torch.equal(y[0], torch.zeros_like(y[0]))
+        assert rel(y[1], orthogonalise(x[1], eps=eps)) <= TOL[dtype]
+
+
+@pytest.mark.parametrize("eps", [1e-7, 1e-20, 0.0])
+def test_muon_leaves_a_layer_without_updates_alone(cuda_device, eps):
+    for shape in ((24, 40), (150, 200)):
+        ps, gs, ms = leaves([shape] * 2)
+        gs[0].zero_()
+        ms[0].zero_()
+        before = ps[0].clone()
+        dcn.muon_update_(ps, gs, ms, lr=0.1, eps=eps)
+        assert torch.equal(ps[0], before) and not ms[0].any() and ps[1].isfinite().all()
