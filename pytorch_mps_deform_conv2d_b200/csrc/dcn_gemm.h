@@ -30,7 +30,7 @@ enum GemmEpilogue {
   // large products compute the upper triangle of tiles and mirror it
   kEpiTerms = 0,
   // the same of v = (diag on the diagonal) + lin * L + acc * factor, L the
-  // two-term matrix `lin16` of the same layout
+  // matrix `lin16` of the same layout and terms
   kEpiPoly = 1,
   // v = acc * scale[b] * factor into `out` of type `out_type`, dense rows of N
   kEpiOut = 2,

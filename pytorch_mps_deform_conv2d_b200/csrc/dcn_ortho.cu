@@ -414,7 +414,8 @@ cudaError_t launch_ortho(const OrthoShape& s, const OrthoChunk& c, void* workspa
     // ones have more steps to come).  1024 x 1024 bf16, relative error before
     // the result's rounding 0.6e-3 -> 1.1e-3, behind it 1.76e-3 -> 1.96e-3
     // (1.66e-3 for an exact result); half of the operations of those steps.
-    sq_terms = s.later_terms == 1 && run == 1 && !first ? 1 : 2;
+    // The chain kernel takes two terms, whatever the run's length.
+    sq_terms = l.m > kChainMax && s.later_terms == 1 && run == 1 && !first ? 1 : 2;
     const GemmOperand X{x[cur], s.rows, s.cols, l.xpitch, terms, l.xterm, c.count,
                         terms * l.xterm, !l.wide};
     const float xs = first ? 1.f : 1.f / later_scale;

@@ -356,3 +356,29 @@ def test_muon_leaves_a_layer_without_updates_alone(cuda_device, eps):
         before = ps[0].clone()
         dcn.muon_update_(ps, gs, ms, lr=0.1, eps=eps)
         assert torch.equal(ps[0], before) and not ms[0].any() and ps[1].isfinite().all()
+
+
+@pytest.mark.parametrize("tf32", [False, True])
+def test_a_last_run_of_one_step_on_few_directions(cuda_device, tf32):
+    # Two runs of one step (13^2 ends the first).  S is 0.7327 in the first, where
+    # fp16 leaves a low term of 2^-13, and 2.9e-4 in the second, whose polynomial
+    # 0.01 + 15 S would take a quarter of its value from a low term of the first.
+    # p(S) of the first, 0.02, is the difference of terms of 13 to 2^-22: 2e-4
+    coef, eps = [(13.0, -15.0, -3.7072), (0.01, 15.0, 0.0)], 0.67312
+    x = torch.ones(1, 16, device="cuda", dtype=torch.float32 if tf32 else torch.bfloat16)
+    if tf32:
+        dcn.set_math_mode("tf32")
+    try:
+        y = dcn.newton_schulz(x, steps=2, coefficients=coef, eps=eps)
+    finally:
+        dcn.set_math_mode(None)
+    assert rel(y, orthogonalise(x, 2, coef, eps)) <= TOL[torch.bfloat16]
+
+
+@pytest.mark.parametrize("steps", [4, 6, 7, 10])
+@pytest.mark.parametrize("shape", [(64, 576), (100, 48), (128, 300), (200, 900)], ids=str)
+def test_steps_of_16_bit_results(cuda_device, shape, steps):
+    # 4, 7 and 10 steps end in a run of one
+    for dtype in (torch.bfloat16, torch.float16):
+        x = gradient(*shape, dtype=dtype)
+        assert rel(dcn.newton_schulz(x, steps=steps), orthogonalise(x, steps)) <= TOL[dtype]
