@@ -764,9 +764,9 @@ cudaError_t launch_quantize_rows(const void* x, int type, long long rows, int co
     auto kern8 = type == kF32 ? quantize_rows8_kernel<kF32>
                  : type == kBF16T ? quantize_rows8_kernel<kBF16T>
                                   : quantize_rows8_kernel<kF16T>;
-    const int vecs = cols / 8, warps = (vecs + 31) / 32;
-    kern8<<<(unsigned)rows, 32 * (warps < 8 ? warps : 8), 0, stream>>>(x, vecs, ldx, q, ldq,
-                                                                       scale);
+    // (rows without columns take a warp too: their scale is 0)
+    const int vecs = cols / 8, need = (vecs + 31) / 32, warps = need < 1 ? 1 : need < 8 ? need : 8;
+    kern8<<<(unsigned)rows, 32 * warps, 0, stream>>>(x, vecs, ldx, q, ldq, scale);
     return cudaGetLastError();
   }
   auto kern = type == kF32 ? quantize_rows_kernel<kF32>

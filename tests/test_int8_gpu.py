@@ -391,3 +391,12 @@ def test_waits_that_run_out_over_many_tiles_are_reported(cuda_device, tokens, ci
     assert dcn.device_status() & STATUS_DENSE_TIMEOUT
     check_linear(dcn.int8_linear(q, w, s, x_scale=xs), q, xs, w, s, None)
     dcn.check_device_status()
+
+
+def test_rows_without_columns_have_scale_zero(cuda_device):
+    lib = _native.load_capi()
+    for t in range(3):  # DCN_TYPE_F32, BF16, F16
+        s = torch.full((5,), 7.0, device="cuda")
+        assert lib.dcn_quantize_int8(5, 0, t, None, None, s.data_ptr(),
+                                     torch.cuda.current_stream().cuda_stream) == 0
+        assert not s.any()
