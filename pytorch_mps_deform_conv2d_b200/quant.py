@@ -9,6 +9,7 @@ counterpart.
 """
 from __future__ import annotations
 
+import copy
 from typing import Optional, Tuple
 
 import torch
@@ -77,8 +78,9 @@ def deform_conv2d_int8(input: Tensor, offset: Tensor, weight: Tensor, weight_sca
 
 class Int8DeformConv2d(nn.Module):
     """A trained :class:`DeformConv2d` or :class:`DeformConv2dPack` in 8 bits
-    (:meth:`from_float`): the codes and scales of its weight as buffers, the
-    bias and a pack's ``conv_offset`` as they were."""
+    (:meth:`from_float`): the codes and scales of its weight as buffers, copies
+    of its bias and of a pack's ``conv_offset``, which stays floating and asks
+    for no gradient."""
 
     def __init__(self, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor], stride,
                  padding, dilation, conv_offset: Optional[nn.Module] = None,
@@ -100,8 +102,10 @@ class Int8DeformConv2d(nn.Module):
         codes, scale = quantize_int8(w.flatten(1))
         bias = None if module.bias is None else module.bias.detach().clone()
         pack = isinstance(module, DeformConv2dPack)
+        # its own: .half() here, or a step of the module's training, stays apart
+        conv_offset = copy.deepcopy(module.conv_offset).requires_grad_(False) if pack else None
         return cls(codes.view(w.shape), scale, bias, module.stride, module.padding,
-                   module.dilation, module.conv_offset if pack else None,
+                   module.dilation, conv_offset,
                    module.deformable_groups if pack else 1, module.modulated if pack else True)
 
     def _apply(self, fn, *args, **kwargs):

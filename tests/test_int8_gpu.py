@@ -400,3 +400,21 @@ def test_rows_without_columns_have_scale_zero(cuda_device):
         assert lib.dcn_quantize_int8(5, 0, t, None, None, s.data_ptr(),
                                      torch.cuda.current_stream().cuda_stream) == 0
         assert not s.any()
+
+
+def test_a_served_pack_is_apart_from_the_trained_one(cuda_device):
+    torch.manual_seed(0)
+    block = dcn.DeformConv2dPack(16, 16, 3, padding=1).cuda()
+    torch.nn.init.normal_(block.conv_offset.weight, std=0.1)
+    served = dcn.Int8DeformConv2d.from_float(block)
+    x = torch.randn(1, 16, 9, 9, device="cuda")
+    y = served(x)
+    with torch.no_grad():
+        for p in block.parameters():
+            p.add_(0.1)
+    assert torch.equal(served(x), y)
+    assert not any(p.requires_grad for p in served.parameters())
+    served.half()
+    assert {p.dtype for p in block.parameters()} == {torch.float32}
+    assert all(p.requires_grad for p in block.parameters())
+    assert served(x.half()).dtype == torch.half
