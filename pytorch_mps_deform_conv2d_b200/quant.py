@@ -26,10 +26,12 @@ def quantize_int8(x: Tensor) -> Tuple[Tensor, Tensor]:
     ``scale = max|x| / 127``, ``code = x / scale`` rounded to the nearest whole
     number (ties to even); a row of zeros gets scale 0.  A row with NaN or an
     infinity gets that as its scale and zeros, so that its products are NaN.
-    A weight (outC, ...) is quantised as ``quantize_int8(weight.flatten(1))``.
+    A weight (outC, ...) is quantised as
+    ``quantize_int8(weight.detach().flatten(1))``.  Not differentiable.
     """
     _cuda_only("x", "quantize_int8", x)
-    return _ops().quantize_int8.default(x.detach() if x.requires_grad else x)
+    _no_grad_only("quantize_int8", x)
+    return _ops().quantize_int8.default(x)
 
 
 def int8_linear(x: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor] = None,
@@ -80,7 +82,7 @@ class Int8DeformConv2d(nn.Module):
     """A trained :class:`DeformConv2d` or :class:`DeformConv2dPack` in 8 bits
     (:meth:`from_float`): the codes and scales of its weight as buffers, copies
     of its bias and of a pack's ``conv_offset``, which stays floating and asks
-    for no gradient."""
+    for no gradient.  Inputs that ask for one are refused."""
 
     def __init__(self, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor], stride,
                  padding, dilation, conv_offset: Optional[nn.Module] = None,
@@ -119,12 +121,7 @@ class Int8DeformConv2d(nn.Module):
     def forward(self, input: Tensor, offset: Optional[Tensor] = None,
                 mask: Optional[Tensor] = None,
                 out_dtype: Optional[torch.dtype] = None) -> Tensor:
-        if torch.is_grad_enabled():
-            with torch.no_grad():
-                return self._forward(input, offset, mask, out_dtype)
-        return self._forward(input, offset, mask, out_dtype)
-
-    def _forward(self, input, offset, mask, out_dtype):
+        _no_grad_only("Int8DeformConv2d", input, offset, mask)
         logits = False
         if self.conv_offset is not None:
             if offset is not None or mask is not None:

@@ -180,3 +180,12 @@ def test_sides_that_tiles_would_round_past_31_bits_are_refused():
     for n in (top + 1, (1 << 31) - 1):
         assert lib.dcn_newton_schulz_workspace_size(1, 1, n, F32, 1, 0) == 0
         assert lib.dcn_muon_update_workspace_size(1, n, 1, F32, 1, 0) == 0
+
+
+def test_int8_module_refuses_gradients():
+    m = dcn.Int8DeformConv2d(torch.zeros(4, 2, 3, 3, dtype=torch.int8), torch.rand(4), None, 1, 1, 1)
+    x, off = torch.randn(1, 2, 5, 5, requires_grad=True), torch.zeros(1, 18, 5, 5)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        m(x, off)
+    with torch.no_grad(), pytest.raises(NotImplementedError, match="CUDA"):
+        m(x, off)

@@ -418,3 +418,29 @@ def test_a_served_pack_is_apart_from_the_trained_one(cuda_device):
     assert {p.dtype for p in block.parameters()} == {torch.float32}
     assert all(p.requires_grad for p in block.parameters())
     assert served(x.half()).dtype == torch.half
+
+
+@pytest.mark.parametrize("modulated", [True, False])
+def test_gradients_are_refused_not_dropped(cuda_device, modulated):
+    x = torch.randn(1, 8, 7, 7, device="cuda")
+    leaf = x.clone().requires_grad_()
+    block = dcn.DeformConv2dPack(8, 8, 3, padding=1, modulated=modulated).cuda()
+    served = dcn.Int8DeformConv2d.from_float(block)
+    plain = dcn.Int8DeformConv2d.from_float(dcn.DeformConv2d(8, 8, 3, padding=1).cuda())
+    # (a conv_offset that asks for gradients, given by hand)
+    own = dcn.Int8DeformConv2d(served.weight, served.weight_scale, served.bias, 1, 1, 1,
+                               block.conv_offset, modulated=modulated)
+    off = torch.zeros(1, 18, 7, 7, device="cuda")
+    mask = torch.ones(1, 9, 7, 7, device="cuda")
+    calls = (lambda: served(leaf), lambda: own(x), lambda: plain(leaf, off),
+             lambda: plain(x, off.clone().requires_grad_()),
+             lambda: plain(x, off, mask.clone().requires_grad_()),
+             lambda: dcn.quantize_int8(block.weight.flatten(1)))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    with torch.no_grad():
+        assert torch.equal(own(x), served(leaf))
+    assert not served(x).requires_grad
