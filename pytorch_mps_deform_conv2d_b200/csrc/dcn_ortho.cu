@@ -22,6 +22,8 @@
 // diverges on steep spectra.
 #include "dcn_ortho.h"
 
+#include <cmath>
+
 #include "dcn_capi_util.h"
 #include "dcn_dense_common.cuh"
 #include "dcn_launch.h"
@@ -414,8 +416,12 @@ cudaError_t launch_ortho(const OrthoShape& s, const OrthoChunk& c, void* workspa
     // ones have more steps to come).  1024 x 1024 bf16, relative error before
     // the result's rounding 0.6e-3 -> 1.1e-3, behind it 1.76e-3 -> 1.96e-3
     // (1.66e-3 for an exact result); half of the operations of those steps.
-    // The chain kernel takes two terms, whatever the run's length.
-    sq_terms = l.m > kChainMax && s.later_terms == 1 && run == 1 && !first ? 1 : 2;
+    // What S loses reaches P times |b| + 2 |c|, 8.9 for the usual coefficients;
+    // larger ones keep two terms (4.125, -11.75, 8.5 on 300 x 500 bf16: 4.5e-3
+    // with one).  So do few directions: the chain kernel takes two.
+    const float* abc0 = s.coef + 3 * k;
+    const bool mild = std::fabs(abc0[1]) + 2.f * std::fabs(abc0[2]) <= 9.f;
+    sq_terms = l.m > kChainMax && s.later_terms == 1 && run == 1 && !first && mild ? 1 : 2;
     const GemmOperand X{x[cur], s.rows, s.cols, l.xpitch, terms, l.xterm, c.count,
                         terms * l.xterm, !l.wide};
     const float xs = first ? 1.f : 1.f / later_scale;

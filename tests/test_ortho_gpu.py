@@ -382,3 +382,36 @@ def test_steps_of_16_bit_results(cuda_device, shape, steps):
     for dtype in (torch.bfloat16, torch.float16):
         x = gradient(*shape, dtype=dtype)
         assert rel(dcn.newton_schulz(x, steps=steps), orthogonalise(x, steps)) <= TOL[dtype]
+
+
+def fp16_between(u, coef, squares):
+    """The choice made for bf16 results, in 64 bits: X as one fp16 term between
+    single steps, with `squares` S and P of all but the first two as well."""
+    def half(x, scale):
+        return (x * scale).half().double() / scale
+
+    x = u.double() / (u.double().norm() + 1e-7)
+    flip = x.shape[0] > x.shape[1]
+    x = x.mT if flip else x
+    for i, (a, b, c) in enumerate(coef):
+        cut = (lambda t: half(t, 1024.0)) if squares and i > 1 else (lambda t: t)
+        s = cut(x @ x.mT)
+        p = cut(a * torch.eye(len(s), dtype=s.dtype, device=s.device) + b * s + c * (s @ s))
+        x = p @ x
+        if i + 1 < len(coef):
+            x = half(x, 1024.0)
+    return x.mT if flip else x
+
+
+@pytest.mark.parametrize("coef,squares", [([COEF] * 5, True), ([(4.125, -11.75, 8.5)] * 5, False),
+                                          ([(4.5, -14.0, 10.0)] * 4, False)], ids=str)
+@pytest.mark.parametrize("shape", [(300, 500), (520, 520), (700, 400)], ids=str)
+def test_bf16_results_are_off_by_the_roundings_chosen_for_them(cuda_device, shape, coef, squares):
+    # Those of X, S and P, and the result's own, are independent: their squares
+    # add.  A quarter more for where the roundings fall.  (S and P keep two terms
+    # for coefficients that would multiply their roundings.)
+    x = gradient(*shape, dtype=torch.bfloat16)
+    want = orthogonalise(x, len(coef), coef)
+    chosen, own = rel(fp16_between(x, coef, squares), want), rel(want.bfloat16(), want)
+    got = dcn.newton_schulz(x, steps=len(coef), coefficients=coef)
+    assert rel(got, want) <= (own ** 2 + (1.25 * chosen) ** 2) ** 0.5
