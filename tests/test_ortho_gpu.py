@@ -415,3 +415,19 @@ def test_bf16_results_are_off_by_the_roundings_chosen_for_them(cuda_device, shap
     chosen, own = rel(fp16_between(x, coef, squares), want), rel(want.bfloat16(), want)
     got = dcn.newton_schulz(x, steps=len(coef), coefficients=coef)
     assert rel(got, want) <= (own ** 2 + (1.25 * chosen) ** 2) ** 0.5
+
+
+@pytest.mark.parametrize("shape", [(2304, 2304), (2570, 2304), (2304, 7000)], ids=str)
+def test_products_of_sm_pairs_with_mirrored_halves(cuda_device, shape):
+    # Gram matrices from some 2200 rows take 256 x 256 tiles on two SMs and write
+    # both halves: one-term squares for bf16 (two terms where X is long), two for
+    # float16
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        x = gradient(*shape, dtype=dtype)
+        want = orthogonalise(x)
+        bound = TOL[dtype]
+        if dtype == torch.bfloat16:
+            chosen, own = rel(fp16_between(x, [COEF] * 5, True), want), rel(want.bfloat16(), want)
+            bound = (own ** 2 + (1.25 * chosen) ** 2) ** 0.5
+        assert rel(dcn.newton_schulz(x), want) <= bound, dtype
+    assert dcn.device_status() == 0
