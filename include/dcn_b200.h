@@ -334,8 +334,9 @@ DCN_API int dcn_h16_staging(const dcn_shape* shape, uint32_t flags);
  * matrices keep what their type can hold.  A matrix of zeros stays zero for any
  * eps; one with NaN or an infinity gives NaN everywhere.  Made for polynomials that keep singular values of
  * [0, 1] below 2: S is held up to 8, a I + b S + c S S up to 16; beyond, results
- * may be NaN.  At most 32 steps, coefficients of 15, 2^31 - 1 elements, a
- * larger side of 2^31 - 256 and a smaller one of 32768. */
+ * may be NaN.  At most 32 steps, a of 15 in size and either b and c or the
+ * polynomial's values for S in [0, 1] too, 2^31 - 1 elements, a larger side of
+ * 2^31 - 256 and a smaller one of 32768. */
 DCN_API size_t dcn_newton_schulz_workspace_size(int64_t count, int64_t rows, int64_t cols,
                                                 int type, int steps, uint32_t flags);
 DCN_API int dcn_newton_schulz(int64_t count, int64_t rows, int64_t cols, int type,

@@ -52,6 +52,18 @@ struct Carve {
   }
 };
 
+// The polynomial a + b S + c S S is summed in fp32 and its values are stored in
+// fp16 (up to 16): those on [0, 1] have to fit, b and c by themselves need not.
+bool polynomial_fits(const float* abc) {
+  const double a = abc[0], b = abc[1], c = abc[2], most = 15.0;
+  if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c) || std::fabs(a) > most)
+    return false;
+  if (std::fabs(b) <= most && std::fabs(c) <= most) return true;
+  const double turn = c != 0.0 ? -b / (2.0 * c) : -1.0;  // of the parabola
+  return std::fabs(a + b + c) <= most &&
+         (turn <= 0.0 || turn >= 1.0 || std::fabs(a + 0.5 * b * turn) <= most);
+}
+
 // fp16 terms by what the result can hold: bf16 keeps 8 bits, so X between two
 // runs is rounded to fp16's 11 once; fp16 and fp32 results take both terms
 // there.  fp32 tensors under DCN_MATH_TF32 ask for 11 bits.
@@ -77,9 +89,10 @@ int ortho_shape(int64_t rows, int64_t cols, int type, int steps, const float* co
   s.eps = eps;
   if (coef != nullptr) {
     std::memcpy(s.coef, coef, sizeof(float) * 3 * steps);
-    for (int i = 0; i < 3 * steps; ++i)
-      DCN_CHECK(std::isfinite(s.coef[i]) && std::fabs(s.coef[i]) <= 15.f,
-                "%s: coefficients must be finite and at most 15 in size", op);
+    for (int i = 0; i < steps; ++i)
+      DCN_CHECK(polynomial_fits(coef + 3 * i),
+                "%s: coefficients (a, b, c) must be finite, a at most 15 in size, and b and c, or "
+                "the values of a + b s + c s^2 for s in [0, 1], too", op);
   }
   return DCN_OK;
 }

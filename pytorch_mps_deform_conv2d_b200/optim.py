@@ -49,8 +49,9 @@ def newton_schulz(update: Tensor, steps: int = 5, coefficients: Coefficients = C
 
     ``steps`` times ``X <- a X + (b S + c S S) X`` with ``S = X X^T`` (of the
     smaller side), from ``X = update / (norm + eps)`` with the Frobenius norm;
-    ``coefficients`` is ``(a, b, c)`` or one triple a step (each value at most
-    15 in size), of polynomials that keep singular values of [0, 1] below 2
+    ``coefficients`` is ``(a, b, c)`` or one triple a step (``a`` at most 15 in
+    size, ``b`` and ``c`` too or else ``a + b s + c s^2`` for ``s`` in [0, 1]),
+    of polynomials that keep singular values of [0, 1] below 2
     (others may end in NaN).  float32, bfloat16 or float16 in and out, any strides; the
     result is contiguous.  float32 keeps fp32 accuracy, or about that of TF32
     in the math mode ``"tf32"`` (:func:`set_math_mode`).  A matrix of zeros

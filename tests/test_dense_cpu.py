@@ -189,3 +189,20 @@ def test_int8_module_refuses_gradients():
         m(x, off)
     with torch.no_grad(), pytest.raises(NotImplementedError, match="CUDA"):
         m(x, off)
+
+
+def test_polynomials_that_fit_are_taken():
+    # by the values on [0, 1], whatever b and c are (the last refused by its workspace)
+    lib = _native.load_capi()
+
+    def call(*abc):
+        return lib.dcn_newton_schulz(1, 64, 128, F32, P, P, 1, coef(*abc), 0.0, 0, P, 16, None)
+
+    for abc in ((8.25, -23.5, 17.0), (15, 15, 15), (15, -30, 0), (-15, 30, 0), (0, 60, -60),
+                (15, -120, 120)):
+        assert call(*abc) == WORKSPACE, abc
+    inf, nan = float("inf"), float("nan")
+    for abc in ((15.1, 0, 0), (-16, 20, 0), (15, 16, 0), (0, 64, -64), (15, -125, 125), (3, 0, 20),
+                (1, inf, 0), (1, -inf, inf), (1, nan, 0), (1, 0, nan), (3, 1e38, -1e38)):
+        assert call(*abc) == INVALID, abc
+    assert b"at most 15" in lib.dcn_last_error()

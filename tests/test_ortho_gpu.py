@@ -431,3 +431,16 @@ def test_products_of_sm_pairs_with_mirrored_halves(cuda_device, shape):
             bound = (own ** 2 + (1.25 * chosen) ** 2) ** 0.5
         assert rel(dcn.newton_schulz(x), want) <= bound, dtype
     assert dcn.device_status() == 0
+
+
+@pytest.mark.parametrize("shape", [(64, 576), (200, 300), (300, 900), (900, 300)], ids=str)
+def test_schedules_of_steep_polynomials(cuda_device, shape):
+    # first steps whose b and c are beyond 15; singular values stay below 2.  Errors
+    # of S reach P times |b| + 2 |c| = 58 in the first step, 9 at most in the others
+    # and in the usual schedule: 6.5 times its bound for float32
+    coef = [(8.25, -23.5, 17.0), (4.1, -2.95, 0.545), (3.95, -2.9, 0.55), (3.3, -2.45, 0.5),
+            (2.3, -1.65, 0.42)]
+    for dtype in DTYPES:
+        x = gradient(*shape, dtype=dtype)
+        bound = 6.5 * F32 + (0 if dtype == torch.float32 else TOL[dtype])
+        assert rel(dcn.newton_schulz(x, coefficients=coef), orthogonalise(x, 5, coef)) <= bound
