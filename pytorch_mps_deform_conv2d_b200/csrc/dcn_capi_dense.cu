@@ -108,6 +108,7 @@ struct DeformInt8 {
   int64_t kg, kp;  // columns a group, padded
   int64_t chunk;   // pixels at a time
   bool pack;       // the weight's rows need the padded pitch
+  bool nhwc;       // the image is sampled where it lies
   size_t stage_bytes, col_bytes, scale_bytes, weight_bytes, total;
 };
 
@@ -133,9 +134,10 @@ int deform_int8_plan(const dcn_shape* shape, int type, uint32_t flags, DeformInt
   d.chunk = g.NP;
   const int64_t fit = (int64_t)(kColumnBytes / (size_t)(a_pixel > 0 ? a_pixel : 1)) / 128 * 128;
   if (d.chunk > fit) d.chunk = fit > 128 ? fit : 128;
-  const bool nhwc = flags & DCN_INPUT_NHWC;
-  // the staging kernels append a row of zeros
-  d.stage_bytes = nhwc ? 0 : align_up(((size_t)g.N * g.HW * g.C + g.C) * type_bytes(type));
+  // (images without pixels may have no address: theirs is the row of zeros that
+  // the staging kernels append)
+  d.nhwc = (flags & DCN_INPUT_NHWC) && g.HW > 0;
+  d.stage_bytes = d.nhwc ? 0 : align_up(((size_t)g.N * g.HW * g.C + g.C) * type_bytes(type));
   d.col_bytes = align_up((size_t)d.chunk * a_pixel);
   d.scale_bytes = align_up((size_t)d.chunk * g.G * sizeof(float));
   d.weight_bytes = align_up((size_t)g.outC * d.kp);  // for rows off their pitch or alignment
@@ -405,7 +407,7 @@ DCN_API int dcn_deform_int8(const dcn_shape* shape, int type, const void* input,
             "dcn_deform_int8: output and bias must be float32, bfloat16 or float16");
   DCN_CHECK(g.C > 0, "dcn_deform_int8: at least one input channel is needed");
   if (g.NP == 0 || g.outC == 0) return DCN_OK;
-  DCN_CHECK(input != nullptr && weight != nullptr && weight_scale != nullptr &&
+  DCN_CHECK((input != nullptr || g.HW == 0) && weight != nullptr && weight_scale != nullptr &&
                 offset != nullptr && output != nullptr,
             "dcn_deform_int8: input, weight, weight_scale, offset and output must not be NULL");
   if (workspace == nullptr || workspace_bytes < d.total)
@@ -416,7 +418,7 @@ DCN_API int dcn_deform_int8(const dcn_shape* shape, int type, const void* input,
   float* scale = ws.take<float>(d.scale_bytes);
   signed char* wp = ws.take<signed char>(d.weight_bytes);
   const void* x = input;
-  if (!(flags & DCN_INPUT_NHWC)) {
+  if (!d.nhwc) {
     if (type == DCN_TYPE_F32)
       DCN_CUDA(dcn::launch_nchw_to_nhwc(static_cast<const float*>(input), static_cast<float*>(xt),
                                         g.N, g.C, g.HW, true, nullptr, stream),

@@ -9,6 +9,8 @@ that is the division's: the codes equal those of the same fp32 division.  For
 sampled columns some eight roundings of 2^-24 times 127 put at most 127 * 2^-20
 = 1.3e-4 of the codes on the other side; one code in 1.3e-4 of a root mean
 square of 20 and more is 6e-4 of a result."""
+import ctypes
+
 import pytest
 import torch
 
@@ -444,3 +446,34 @@ def test_gradients_are_refused_not_dropped(cuda_device, modulated):
     with torch.no_grad():
         assert torch.equal(own(x), served(leaf))
     assert not served(x).requires_grad
+
+
+@pytest.mark.parametrize("dtype", FLOATS, ids=str)
+@pytest.mark.parametrize("h,w", [(0, 5), (5, 0), (0, 0)])
+def test_images_without_pixels_answer_with_the_bias(cuda_device, h, w, dtype):
+    # all padding, as deform_conv2d takes them
+    torch.manual_seed(0)
+    x = torch.empty(2, 4, h, w, device="cuda", dtype=dtype)
+    off = torch.randn(2, 18, h + 2, w + 2, device="cuda").to(dtype)
+    mask, b = torch.rand(2, 9, h + 2, w + 2, device="cuda").to(dtype), torch.randn(6, device="cuda")
+    wq, ws = rand_codes(6, 4, 3, 3), torch.rand(6, device="cuda")
+    want = b.to(dtype)[None, :, None, None].expand(2, 6, h + 2, w + 2)
+    got = dcn.deform_conv2d_int8(x, off, wq, ws, b, padding=2, mask=mask)
+    assert torch.equal(got, want)
+    if dtype == torch.float32:
+        assert torch.equal(dcn.deform_conv2d(x, off, wq.float(), b, padding=2, mask=mask), want)
+    # the C entry point, told that they lie channels last
+    lib = _native.load_capi()
+    s = _native.DcnShape(batch=2, in_channels=4, height=h, width=w, out_channels=6, kernel_h=3,
+                         kernel_w=3, stride_h=1, stride_w=1, pad_h=2, pad_w=2, dilation_h=1,
+                         dilation_w=1, groups=1, deformable_groups=1)
+    t, flags = FLOATS.index(dtype), 0x20000  # DCN_INPUT_NHWC
+    out = torch.empty_like(got)
+    ws_bytes = lib.dcn_deform_int8_workspace_size(ctypes.byref(s), t, flags)
+    space = torch.empty(ws_bytes, dtype=torch.uint8, device="cuda")
+    wl = wq.permute(0, 2, 3, 1).contiguous()
+    assert lib.dcn_deform_int8(ctypes.byref(s), t, None, wl.data_ptr(), ws.data_ptr(), off.data_ptr(),
+                               mask.data_ptr(), b.data_ptr(), 0, out.data_ptr(), t, flags,
+                               space.data_ptr(), ws_bytes,
+                               torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out, want)
