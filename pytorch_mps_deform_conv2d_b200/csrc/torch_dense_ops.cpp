@@ -12,6 +12,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <iterator>
 #include <utility>
 #include <vector>
 
@@ -139,6 +140,18 @@ void muon_update_(at::TensorList params, at::TensorList grads, at::TensorList mo
     TORCH_CHECK(written[i].first >= written[i - 1].second,
                 "muon_update_: params and momenta must not overlap (the same parameter or "
                 "momentum is given twice?)");
+  for (size_t i = 0; i < grads.size(); ++i) {  // read after the first of them are written
+    const auto& g = grads[i];
+    if (g.numel() == 0) continue;
+    int64_t span = 1;
+    for (int64_t d = 0; d < g.dim(); ++d) span += (g.size(d) - 1) * g.stride(d);
+    const char* gb = static_cast<const char*>(g.data_ptr());
+    const char* ge = gb + span * g.element_size();
+    const auto next = std::lower_bound(written.begin(), written.end(), std::make_pair(gb, gb));
+    TORCH_CHECK((next == written.end() || next->first >= ge) &&
+                    (next == written.begin() || std::prev(next)->second <= gb),
+                "muon_update_: grads must not overlap params or momenta");
+  }
   c10::cuda::CUDAGuard guard(params[0].device());
   std::vector<bool> done(params.size(), false);
   const auto stream = at::cuda::getCurrentCUDAStream().stream();

@@ -444,3 +444,17 @@ def test_schedules_of_steep_polynomials(cuda_device, shape):
         x = gradient(*shape, dtype=dtype)
         bound = 6.5 * F32 + (0 if dtype == torch.float32 else TOL[dtype])
         assert rel(dcn.newton_schulz(x, coefficients=coef), orthogonalise(x, 5, coef)) <= bound
+
+
+def test_muon_refuses_grads_that_it_would_write(cuda_device):
+    whole, p, g = (torch.randn(24, 16, device="cuda") for _ in range(3))
+    before, held = p.clone(), g.clone()
+    z = torch.zeros_like(p)
+    for params, grads, momenta in (([p], [g], [g]), ([p], [p], [z]), ([p, g], [z, p], [whole, z[:]]),
+                                   ([p, whole[:8]], [g, whole[7:15]], [z, z.new_zeros(8, 16)]),
+                                   ([whole[8:16]], [whole[1:24:3]], [z.new_zeros(8, 16)])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            dcn.muon_update_(params, grads, momenta, lr=0.1)
+    assert torch.equal(p, before) and torch.equal(g, held)
+    # neighbours, and one gradient for two
+    dcn.muon_update_([whole[:8], whole[16:]], [whole[8:16]] * 2, list(z.new_zeros(2, 8, 16)), lr=0.1)
