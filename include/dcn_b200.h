@@ -360,6 +360,14 @@ DCN_API int dcn_muon_update(int64_t count, int64_t rows, int64_t cols, int type,
                             float update_scale, int steps, const float* coefficients, float eps,
                             uint32_t flags, void* workspace, size_t workspace_bytes,
                             void* stream);
+/* The same with its settings in double.  1 - momentum is rounded by itself there:
+ * of a float 0.999 it is 1.3e-5 off. */
+DCN_API int dcn_muon_update_f64(int64_t count, int64_t rows, int64_t cols, int type,
+                                void* const* params, const void* const* grads,
+                                float* const* momenta, double lr, double momentum, int nesterov,
+                                double weight_decay, double update_scale, int steps,
+                                const float* coefficients, float eps, uint32_t flags,
+                                void* workspace, size_t workspace_bytes, void* stream);
 
 /* 8-bit codes of dense rows (no reference counterpart): scale = max |x| / 127
  * of the row, code = x / scale rounded to the nearest whole number, ties to

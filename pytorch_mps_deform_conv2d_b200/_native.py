@@ -124,6 +124,10 @@ def load_capi():
         lib.dcn_muon_update.argtypes = ([i64] * 3 + [i32, vpp, vpp, vpp, f32, f32, i32, f32, f32,
                                                      i32, fp, f32, u32, vp, sz, vp])
         lib.dcn_muon_update.restype = i32
+        f64 = ctypes.c_double
+        lib.dcn_muon_update_f64.argtypes = ([i64] * 3 + [i32, vpp, vpp, vpp, f64, f64, i32, f64,
+                                                         f64, i32, fp, f32, u32, vp, sz, vp])
+        lib.dcn_muon_update_f64.restype = i32
         lib.dcn_quantize_int8.argtypes = [i64, i64, i32, vp, vp, vp, vp]
         lib.dcn_quantize_int8.restype = i32
         lib.dcn_int8_linear_workspace_size.argtypes = [i64] * 3 + [i32]

@@ -234,7 +234,18 @@ DCN_API int dcn_muon_update(int64_t count, int64_t rows, int64_t cols, int type,
                             float lr, float momentum, int nesterov, float weight_decay,
                             float update_scale, int steps, const float* coefficients, float eps,
                             uint32_t flags, void* workspace, size_t workspace_bytes,
-                            void* stream_) {
+                            void* stream) {
+  return dcn_muon_update_f64(count, rows, cols, type, params, grads, momenta, lr, momentum,
+                             nesterov, weight_decay, update_scale, steps, coefficients, eps, flags,
+                             workspace, workspace_bytes, stream);
+}
+
+DCN_API int dcn_muon_update_f64(int64_t count, int64_t rows, int64_t cols, int type,
+                                void* const* params, const void* const* grads,
+                                float* const* momenta, double lr, double momentum, int nesterov,
+                                double weight_decay, double update_scale, int steps,
+                                const float* coefficients, float eps, uint32_t flags,
+                                void* workspace, size_t workspace_bytes, void* stream_) {
   g_last_error.clear();
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   dcn::OrthoShape s;
@@ -243,7 +254,7 @@ DCN_API int dcn_muon_update(int64_t count, int64_t rows, int64_t cols, int type,
                        "dcn_muon_update");
   if (rc != DCN_OK) return rc;
   DCN_CHECK(count >= 0, "dcn_muon_update: count must be non-negative");
-  DCN_CHECK(momentum >= 0.f && momentum < 1.f, "dcn_muon_update: momentum must be in [0, 1)");
+  DCN_CHECK(momentum >= 0.0 && momentum < 1.0, "dcn_muon_update: momentum must be in [0, 1)");
   if (count == 0 || rows == 0 || cols == 0) return DCN_OK;
   DCN_CHECK(params != nullptr && grads != nullptr && momenta != nullptr,
             "dcn_muon_update: params, grads and momenta must not be NULL");
@@ -256,9 +267,10 @@ DCN_API int dcn_muon_update(int64_t count, int64_t rows, int64_t cols, int type,
   dcn::OrthoChunk c{};
   c.muon = true;
   c.nesterov = nesterov != 0;
-  c.beta = momentum;
-  c.keep = (float)(1.0 - (double)lr * weight_decay);
-  c.step = (float)(-(double)lr * update_scale);
+  c.beta = (float)momentum;
+  c.rest = (float)(1.0 - momentum);
+  c.keep = (float)(1.0 - lr * weight_decay);
+  c.step = (float)(-lr * update_scale);
   for (int64_t b = 0; b < count; b += chunk) {
     c.count = (int)(count - b < chunk ? count - b : chunk);
     for (int i = 0; i < c.count; ++i) {

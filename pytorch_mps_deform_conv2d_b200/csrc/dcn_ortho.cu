@@ -50,7 +50,7 @@ struct PrepArgs {
   long long numel, pitch, term_stride, batch_stride;
   int rows, cols, type, terms, target;  // |stored X| lies in [2^target, 2^(target + 1))
   int muon, nesterov, vec, partials;
-  float beta, eps;
+  float beta, rest, eps;
 };
 
 template <int T>
@@ -83,7 +83,7 @@ __device__ __forceinline__ void load8(const void* p, long long i, float (&v)[8])
 
 // The update's value from the gradient and the new momentum.
 __device__ __forceinline__ float update_of(const PrepArgs& a, float g, float m) {
-  return a.nesterov ? (1.f - a.beta) * g + a.beta * m : m;
+  return a.nesterov ? a.rest * g + a.beta * m : m;
 }
 
 // New momentum, and sums of squares of the update in 64 bits: any fp32 input
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) ortho_norm_kernel(const __grid_constant__
       float m[8];
       load8<kF32>(mom, 8 * q, m);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m[j] = a.beta * m[j] + (1.f - a.beta) * v[j];
+      for (int j = 0; j < 8; ++j) m[j] = a.beta * m[j] + a.rest * v[j];
       float4* o = reinterpret_cast<float4*>(mom + 8 * q);
       o[0] = make_float4(m[0], m[1], m[2], m[3]);
       o[1] = make_float4(m[4], m[5], m[6], m[7]);
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(256) ortho_norm_kernel(const __grid_constant__
   for (long long i = 8 * vecs + first; i < a.numel; i += step) {
     float v = load1<T>(in, i);
     if (a.muon) {
-      const float m = a.beta * mom[i] + (1.f - a.beta) * v;
+      const float m = a.beta * mom[i] + a.rest * v;
       mom[i] = m;
       v = update_of(a, v, m);
     }
@@ -329,6 +329,7 @@ cudaError_t launch_ortho(const OrthoShape& s, const OrthoChunk& c, void* workspa
   p.muon = c.muon;
   p.nesterov = c.nesterov;
   p.beta = c.beta;
+  p.rest = c.rest;
   p.eps = s.eps;
   p.vec = 1;
   for (int i = 0; i < c.count; ++i)

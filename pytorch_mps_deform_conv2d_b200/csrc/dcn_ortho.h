@@ -27,11 +27,11 @@ struct OrthoChunk {
   const void* in[kGemmMaxList];   // dense (rows, cols)
   void* out[kGemmMaxList];        // dense (rows, cols)
   // optimiser step: `in` are gradients, `out` parameters, updated in place:
-  // m = beta m + (1 - beta) g, u = nesterov ? (1 - beta) g + beta m : m,
-  // p = keep p + step O(u)
+  // m = beta m + rest g, u = nesterov ? rest g + beta m : m,
+  // p = keep p + step O(u); rest is 1 - beta, rounded by itself
   float* momentum[kGemmMaxList];
   bool muon, nesterov;
-  float beta, keep, step;
+  float beta, rest, keep, step;
 };
 
 size_t ortho_workspace_bytes(const OrthoShape& s, int count);

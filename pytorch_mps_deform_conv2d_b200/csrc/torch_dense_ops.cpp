@@ -184,10 +184,9 @@ void muon_update_(at::TensorList params, at::TensorList grads, at::TensorList mo
     const size_t bytes = dcn_muon_update_workspace_size((int64_t)p.size(), rows, cols, type,
                                                         (int)steps, flags);
     auto ws = scratch(bytes);
-    check_rc(dcn_muon_update((int64_t)p.size(), rows, cols, type, p.data(), g.data(), m.data(),
-                             (float)lr, (float)momentum, nesterov ? 1 : 0, (float)weight_decay,
-                             (float)scale, (int)steps, coef.data(), (float)eps, flags,
-                             ws.get(), bytes, stream));
+    check_rc(dcn_muon_update_f64((int64_t)p.size(), rows, cols, type, p.data(), g.data(), m.data(),
+                                 lr, momentum, nesterov ? 1 : 0, weight_decay, scale, (int)steps,
+                                 coef.data(), (float)eps, flags, ws.get(), bytes, stream));
   }
   for (size_t i = 0; i < params.size(); ++i) {  // written through raw pointers
     params[i].unsafeGetTensorImpl()->bump_version();

@@ -9,6 +9,8 @@ results: half a step of the type, eps / 2, plus for bf16 the one rounding of X
 to fp16 (2^-11) two steps from the end, times a^2 = 11.9 (in single steps X, S
 and P are rounded, each by 2^-12 at most where the largest values lie and 2^-13 in
 the mean: no more than that one in three steps together)."""
+import ctypes
+
 import pytest
 import torch
 
@@ -458,3 +460,28 @@ def test_muon_refuses_grads_that_it_would_write(cuda_device):
     assert torch.equal(p, before) and torch.equal(g, held)
     # neighbours, and one gradient for two
     dcn.muon_update_([whole[:8], whole[16:]], [whole[8:16]] * 2, list(z.new_zeros(2, 8, 16)), lr=0.1)
+
+
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("momentum", [0.0, 0.3, 0.99, 0.999, 0.99999])
+def test_muon_weighs_the_gradient_by_one_minus_momentum(cuda_device, momentum, nesterov):
+    # from a momentum of zeros: (1 - momentum) g, two roundings
+    ps, gs, _ = leaves([(24, 40), (150, 200)])
+    ms = [torch.zeros_like(p) for p in ps]
+    check_step(ps, gs, ms, lr=0.02, momentum=momentum, nesterov=nesterov)
+
+
+def test_muon_c_entry_points_agree(cuda_device):
+    lib = _native.load_capi()
+    c = (ctypes.c_float * 3)(*COEF)
+    ws_bytes = lib.dcn_muon_update_workspace_size(1, 24, 40, 0, 1, 0)
+    space = torch.empty(ws_bytes, dtype=torch.uint8, device="cuda")
+    got = []
+    for fn in (lib.dcn_muon_update, lib.dcn_muon_update_f64):
+        (p,), (g,), (m,) = leaves([(24, 40)])
+        one = lambda t: (ctypes.c_void_p * 1)(t.data_ptr())  # noqa: E731
+        # settings that float holds
+        assert fn(1, 24, 40, 0, one(p), one(g), one(m), 0.25, 0.875, 1, 0.5, 1.5, 1, c, 1e-7, 0,
+                  space.data_ptr(), ws_bytes, torch.cuda.current_stream().cuda_stream) == 0
+        got.append((p, m))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
