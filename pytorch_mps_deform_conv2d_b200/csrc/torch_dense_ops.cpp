@@ -130,6 +130,10 @@ void muon_update_(at::TensorList params, at::TensorList grads, at::TensorList mo
                 "muon_update_: params must be dense with dimension 0 outermost, momenta of the "
                 "same strides");
     if (p.numel() == 0) continue;
+    // a size that is refused is refused before any parameter is written
+    TORCH_CHECK(dcn_muon_update_workspace_size(1, p.size(0) / groups, p.numel() / p.size(0),
+                                               type_code(p.scalar_type()), (int)steps, flags) > 0,
+                dcn_last_error());
     const char *pb = static_cast<const char*>(p.data_ptr()),
                *mb = static_cast<const char*>(m.data_ptr());
     written.emplace_back(pb, pb + p.nbytes());

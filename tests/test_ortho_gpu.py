@@ -485,3 +485,15 @@ def test_muon_c_entry_points_agree(cuda_device):
                   space.data_ptr(), ws_bytes, torch.cuda.current_stream().cuda_stream) == 0
         got.append((p, m))
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+def test_muon_refuses_a_size_before_it_writes_anything(cuda_device):
+    side = 32769  # both sides: beyond what is supported
+    small = torch.randn(8, 16, device="cuda", dtype=torch.bfloat16)
+    large = torch.empty(side, side, device="cuda", dtype=torch.bfloat16)
+    ps, ms = [small, large], [torch.zeros_like(p, dtype=torch.float32) for p in (small, large)]
+    gs = [torch.ones_like(small), small.new_ones(1).expand(side, side)]
+    before = small.clone()
+    with pytest.raises(RuntimeError, match="not supported"):
+        dcn.muon_update_(ps, gs, ms, lr=0.1)
+    assert torch.equal(small, before) and not ms[0].any()
