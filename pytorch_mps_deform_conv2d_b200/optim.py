@@ -99,8 +99,9 @@ class Muon(torch.optim.Optimizer):
     :class:`DeformConv2d`'s ``weight``, not its ``bias``.  A grouped
     convolution's parameter group takes ``groups=...``, so that each group's
     rows are a matrix of their own.  The state is one float32 momentum a
-    parameter.  ``lr`` and the other settings are read when ``step`` is called:
-    a captured CUDA graph keeps those of its capture.
+    parameter, made by its first step, which no CUDA graph can capture.  ``lr``
+    and the other settings are read when ``step`` is called: a captured graph
+    keeps those of its capture.
     """
 
     def __init__(self, params: Iterable, lr: float = 0.02, momentum: float = 0.95,
@@ -160,6 +161,11 @@ class Muon(torch.optim.Optimizer):
                     raise RuntimeError("Muon does not support sparse gradients")
                 state = self.state[p]
                 if "momentum_buffer" not in state:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        # every replay would set it to zero again
+                        del self.state[p]
+                        raise RuntimeError("Muon: make a step before the one that a CUDA graph "
+                                           "captures; the momentum does not exist yet")
                     state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
                 by_device.setdefault(p.device, []).append((p, p.grad, state["momentum_buffer"]))
             for items in by_device.values():

@@ -497,3 +497,23 @@ def test_muon_refuses_a_size_before_it_writes_anything(cuda_device):
     with pytest.raises(RuntimeError, match="not supported"):
         dcn.muon_update_(ps, gs, ms, lr=0.1)
     assert torch.equal(small, before) and not ms[0].any()
+
+
+def test_the_first_step_is_not_captured(cuda_device):
+    # a graph that held the momentum's zeros would start from them in every replay
+    w = torch.nn.Parameter(gradient(24, 40))
+    w.grad = gradient(24, 40, seed=1)
+    opt = dcn.Muon([w], lr=0.1)
+    before = w.detach().clone()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    dcn.newton_schulz(w.detach())  # (the kernels are loaded)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        graph.capture_begin()
+        with pytest.raises(RuntimeError, match="before the one"):
+            opt.step()
+        spare = torch.zeros(1, device="cuda")  # something to capture
+        graph.capture_end()
+    assert torch.equal(w, before) and not opt.state and spare is not None
+    opt.step()
+    assert opt.state[w]["momentum_buffer"].any() and not torch.equal(w, before)
