@@ -384,9 +384,13 @@ DCN_API int dcn_quantize_int8(int64_t rows, int64_t cols, int type, const void* 
  * coded as by dcn_quantize_int8 inside the call.  At most 131071 input
  * features, 2^31 - 256 tokens and as many outputs.  Rows of a multiple of 16 features at 16-byte aligned addresses
  * are read where they lie; others are copied first.  Up to 8 tokens of such
- * rows (x and weight aligned) need no workspace: it may be NULL there. */
+ * rows (x and weight aligned) need no workspace: it may be NULL there, and one
+ * kernel does it all.  dcn_int8_linear_few_tokens says whether that is also the
+ * faster way (1), which a call with a workspace takes by itself. */
 DCN_API size_t dcn_int8_linear_workspace_size(int64_t tokens, int64_t in_features,
                                               int64_t out_features, int x_type);
+DCN_API int dcn_int8_linear_few_tokens(int64_t tokens, int64_t in_features,
+                                       int64_t out_features, int x_type);
 DCN_API int dcn_int8_linear(int64_t tokens, int64_t in_features, int64_t out_features, int x_type,
                             const void* x, const float* x_scale, const int8_t* weight,
                             const float* weight_scale, const void* bias, int bias_type,

@@ -132,6 +132,8 @@ def load_capi():
         lib.dcn_quantize_int8.restype = i32
         lib.dcn_int8_linear_workspace_size.argtypes = [i64] * 3 + [i32]
         lib.dcn_int8_linear_workspace_size.restype = sz
+        lib.dcn_int8_linear_few_tokens.argtypes = [i64] * 3 + [i32]
+        lib.dcn_int8_linear_few_tokens.restype = i32
         lib.dcn_int8_linear.argtypes = ([i64] * 3 + [i32, vp, vp, vp, vp, vp, i32, vp, i32, u32,
                                                      vp, sz, vp])
         lib.dcn_int8_linear.restype = i32

@@ -310,6 +310,15 @@ DCN_API size_t dcn_int8_linear_workspace_size(int64_t tokens, int64_t in_feature
   return linear_plan(tokens, in_features, out_features, x_type).total;
 }
 
+DCN_API int dcn_int8_linear_few_tokens(int64_t tokens, int64_t in_features,
+                                       int64_t out_features, int x_type) {
+  return tokens > 0 && in_features > 0 && out_features > 0 &&
+                 dcn::few_tokens_fit(tokens, in_features) &&
+                 dcn::few_tokens_pay(x_type, tokens, in_features, out_features)
+             ? 1
+             : 0;
+}
+
 DCN_API int dcn_int8_linear(int64_t tokens, int64_t in_features, int64_t out_features, int x_type,
                             const void* x, const float* x_scale, const int8_t* weight,
                             const float* weight_scale, const void* bias, int bias_type,
@@ -335,7 +344,9 @@ DCN_API int dcn_int8_linear(int64_t tokens, int64_t in_features, int64_t out_fea
   LinearPlan p = linear_plan(tokens, in_features, out_features, x_type);
   if (workspace != nullptr && workspace_bytes < p.total)
     return fail(DCN_ERR_WORKSPACE, "dcn_int8_linear: workspace too small");
-  if (dcn::few_tokens_fit(tokens, in_features) && aligned16(x) && aligned16(weight)) {
+  if (dcn::few_tokens_fit(tokens, in_features) && aligned16(x) && aligned16(weight) &&
+      (workspace == nullptr ||
+       dcn::few_tokens_pay(x_type, tokens, in_features, out_features))) {
     DCN_CUDA(dcn::launch_few_tokens(x, x_type, x_scale, (int)tokens, (int)in_features,
                                     (int)out_features,
                                     reinterpret_cast<const signed char*>(weight), weight_scale,

@@ -520,6 +520,7 @@ cudaError_t sample_vec_form(const Geom& g, const void* x, const void* off, const
 // codes in shared memory and gives each warp ROWS rows of the weight: lane l
 // multiplies 16-byte vectors l, l + 32, ... with the four-way integer dot
 // product.  The first vectors are on their way while the tokens are coded.
+// (Where it is the faster way: few_tokens_pay.)
 constexpr int kFewAhead = 8;  // 16-byte weight vectors a lane has on its way
 
 template <int T, int NT, int ROWS>
@@ -779,6 +780,21 @@ cudaError_t launch_quantize_rows(const void* x, int type, long long rows, int co
 bool few_tokens_fit(int64_t tokens, int64_t K) {
   const int64_t nt = tokens <= 1 ? 1 : tokens <= 2 ? 2 : tokens <= 4 ? 4 : 8;
   return tokens <= 8 && K % 16 == 0 && nt * K <= 96 * 1024;
+}
+
+// Against the coder and the tensor-core product behind it, in a graph (us, that
+// way in brackets; 9 tokens stand for it).  Every block codes the tokens, so
+// floating ones cost it tokens * K: 4 of K = 1024 to 4096 outputs 8.2 (8.9), of
+// K = 2304 to 256 10.0 (9.2), of K = 4096 to 1024 14.4 (11.8); 2 of 4096 x 4096
+// 13.8 (15.0); 5 of K = 256 to 256 9.8 (6.3), 8 of 4096 x 4096 26.9 (15.0).  8
+// int8 tokens of 4096 x 4096 10.7 (11.3).  Beyond some 32 MB of weight the dot
+// products lose to the tensor core: 4096 x 16384 with 2 floating tokens 33.9
+// (26.5), with 4 int8 ones 22.2 (22.2), with 8 33.9 (22.2); 8192 x 8192 with 2
+// int8 ones 19.6 (25.2).
+bool few_tokens_pay(int x_type, int64_t tokens, int64_t K, int64_t N) {
+  const bool small = K * N <= (int64_t(32) << 20);
+  if (x_type == 3) return tokens <= 2 || small;
+  return tokens <= 1 || (small && (tokens <= 2 || (tokens <= 4 && tokens * K <= 8192)));
 }
 
 cudaError_t launch_few_tokens(const void* x, int x_type, const float* x_scale, int tokens, int K,

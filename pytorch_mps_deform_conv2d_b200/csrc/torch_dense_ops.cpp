@@ -283,7 +283,8 @@ at::Tensor int8_linear(const at::Tensor& x, const at::Tensor& weight,
                            at::cuda::getCurrentCUDAStream().stream());
   };
   // a few tokens take no workspace where their rows allow it
-  int rc = tokens <= 8 ? call(nullptr) : DCN_ERR_WORKSPACE;
+  int rc = dcn_int8_linear_few_tokens(tokens, in, w.size(0), xt) ? call(nullptr)
+                                                                 : DCN_ERR_WORKSPACE;
   if (rc == DCN_ERR_WORKSPACE) {
     auto ws = scratch(bytes);
     rc = call(ws.get());

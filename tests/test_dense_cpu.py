@@ -206,3 +206,13 @@ def test_polynomials_that_fit_are_taken():
                 (1, inf, 0), (1, -inf, inf), (1, nan, 0), (1, 0, nan), (3, 1e38, -1e38)):
         assert call(*abc) == INVALID, abc
     assert b"at most 15" in lib.dcn_last_error()
+
+
+def test_few_tokens_query():
+    few = _native.load_capi().dcn_int8_linear_few_tokens
+    assert few(1, 4096, 1 << 20, BF16) == 1 and few(2, 8192, 8192, I8) == 1
+    assert few(2, 4096, 4096, F16) == 1 and few(2, 8192, 8192, F16) == 0
+    assert few(4, 1024, 4096, BF16) == 1 and few(4, 4096, 4096, BF16) == 0
+    assert few(8, 4096, 4096, I8) == 1 and few(8, 4096, 4096, F32) == 0
+    # rows that the kernel does not take, more tokens, nothing
+    assert few(1, 4095, 16, BF16) == 0 and few(9, 64, 64, I8) == 0 and few(0, 64, 64, I8) == 0

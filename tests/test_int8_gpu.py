@@ -477,3 +477,25 @@ def test_images_without_pixels_answer_with_the_bias(cuda_device, h, w, dtype):
                                space.data_ptr(), ws_bytes,
                                torch.cuda.current_stream().cuda_stream) == 0
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("given", [True, False])
+@pytest.mark.parametrize("cin,cout", [(64, 40), (1024, 96), (2304, 250), (4096, 1000), (4096, 8200)])
+def test_two_to_nine_tokens_by_either_way(cuda_device, cin, cout, given):
+    # one kernel, or coder and tensor-core product, by sizes; without a workspace
+    # the former up to eight
+    lib = _native.load_capi()
+    w, ws = rand_codes(cout, cin, seed=1), torch.rand(cout, device="cuda") / cin
+    for tokens in range(2, 10):
+        x = torch.randn(tokens, cin, device="cuda").bfloat16()
+        q, xs = dcn.quantize_int8(x)
+        kw = dict(x_scale=xs) if given else {}
+        y = dcn.int8_linear(q if given else x, w, ws, out_dtype=torch.float32, **kw)
+        check_linear(y, q, xs, w, ws, None)
+        if tokens <= 8:
+            z = torch.empty_like(y)
+            a, t, s = (q, 3, xs.data_ptr()) if given else (x, 1, None)
+            assert lib.dcn_int8_linear(tokens, cin, cout, t, a.data_ptr(), s, w.data_ptr(),
+                                       ws.data_ptr(), None, 0, z.data_ptr(), 0, 0, None, 0,
+                                       torch.cuda.current_stream().cuda_stream) == 0
+            check_linear(z, q, xs, w, ws, None)
