@@ -401,8 +401,11 @@ DCN_API int dcn_int8_linear(int64_t tokens, int64_t in_features, int64_t out_fea
  * counterpart).  input, offset and mask of `type` as in dcn_forward; weight
  * int8 in (outC, kh, kw, C/groups) order, a scale for each output channel
  * (rows of a multiple of 16 codes at a 16-byte aligned address are read where
- * they lie, others are copied first).  The sampled columns of each output pixel and group are
- * coded as by dcn_quantize_int8 (a token), their products with the weight
+ * they lie, others are copied first).  The sampled columns of each output pixel
+ * and group are coded as by dcn_quantize_int8 (a token), but times one
+ * reciprocal of their scale: where that and the roundings of the samples put a
+ * value past the middle of two codes, it takes the other.  Their products with
+ * the weight are
  * scaled back.  `flags`: DCN_MASK_LOGITS, DCN_INPUT_NHWC.  The output is dense
  * NCHW of `out_type`.  At most 131071 columns and 2^31 - 256 output channels a
  * group. */

@@ -14,9 +14,9 @@
 // part of it, and every further step of the run multiplies that by a^2 while
 // those values grow.  A run ends before the product of its a^2 passes 150:
 // three steps of the usual 3.4445, two runs for five steps; results of 16 bits
-// do not see the difference (squarer matrices: run_length below).  For fp32 results the first run, where one
-// direction can hold nearly all of |X|, ends before 12: two steps; so does
-// every run of more than 256 directions.  Emulated in 64 bits on 64 x 576 with
+// do not see the difference (squarer matrices: run_length below).  For fp32
+// results the first run, where one direction can hold nearly all of |X|, ends
+// before 12: two steps; so does every run of more than 256 directions.  Emulated in 64 bits on 64 x 576 with
 // a few strong directions, the relative error is 5e-7 with runs (2, 3) and
 // 4.6e-6 with (3, 2), fp32 products as written 1.4e-6; one run of five steps
 // diverges on steep spectra.
@@ -247,10 +247,20 @@ int run_length(const OrthoShape& s, int first) {
   const bool square = m > kChainMax && n < (s.later_terms == 1 ? 3LL : 2LL) * m;
   if (square && (first > 0 || s.later_terms == 2)) return 1;
   // The more directions, and the squarer the matrix, the more of them are still
-  // small in the second run.
-  // Relative errors with runs (2, 3), (2, 2, 1) and of fp32 products: 300 x 2700
-  // 0.85e-6, 1.0e-6, 1.5e-6; 515 x 1153 3.2e-6, 2.0e-6, 2.6e-6; 1400 x 2900
-  // 6.7e-6, 2.7e-6, 3.8e-6.
+  // small in the second run: up to 256 that run may be long, where the error stays
+  // below twice that of fp32 products as written.  From some 350 on it would
+  // pass that, for a twentieth of the time at best.  Relative errors (largest of three gradients
+  // of rank m / 16 under noise), us, with runs (2, 3), with (2, 2, 1), and the
+  // error of fp32 products:
+  //   128 x 1152  0.80e-6  79    0.99e-6  90   1.05e-6  (the chain kernel's)
+  //   192 x 400   2.2e-6  110    1.7e-6  106   1.6e-6
+  //   256 x 520   3.5e-6  127    2.1e-6  130   1.9e-6
+  //   256 x 2304  2.8e-6  132    2.7e-6  136   1.8e-6
+  //   300 x 700   4.1e-6  136    2.3e-6  135   2.2e-6
+  //   300 x 2700  3.4e-6  146    3.0e-6  148   2.1e-6
+  //   384 x 1600  5.2e-6  157    3.1e-6  160   2.7e-6
+  //   512 x 4608  6.7e-6  196    3.7e-6  206   3.4e-6
+  //   1400 x 2900 9.0e-6  594    1.6e-6  611   2.8e-6
   const bool f32 = s.first_terms == 2 && s.later_terms == 2;
   const bool few = f32 ? first == 0 || m > 256 || n < 2LL * m : square;
   const float limit = few ? kShortRunLimit : kRunLimit;

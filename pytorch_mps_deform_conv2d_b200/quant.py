@@ -60,9 +60,15 @@ def deform_conv2d_int8(input: Tensor, offset: Tensor, weight: Tensor, weight_sca
     ``weight_scale`` holds a float32 scale for each output channel; a
     channels-last weight is read where it lies, another is laid out anew in
     every call.  Each output pixel's sampled column is coded as by
-    :func:`quantize_int8` (for each convolution group).  input, offset and mask
-    share one of float32, bfloat16 and float16; ``out_dtype`` defaults to it.
-    ``mask_logits`` as in :func:`deform_conv2d_ex`.
+    :func:`quantize_int8` (for each convolution group), but times one reciprocal
+    of its scale: a value within that rounding of the middle of two codes may
+    take the other.  input, offset and mask share one of float32, bfloat16 and
+    float16; ``out_dtype`` defaults to it.  ``mask_logits`` as in
+    :func:`deform_conv2d_ex`.
+
+    A layer of hundreds of channels takes about the time of
+    :func:`deform_conv2d` in 16 bits, with half of the weight's bytes; groups of
+    a few channels are several times slower than there.
     """
     stride, padding, dilation = _pair(stride), _pair(padding), _pair(dilation)
     _cuda_only("input", "deform_conv2d_int8", input)
