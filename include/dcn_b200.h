@@ -330,13 +330,15 @@ DCN_API int dcn_h16_staging(const dcn_shape* shape, uint32_t flags);
  * from X = G / (|G| + eps), |G| the Frobenius norm; `coefficients` are host
  * memory: (a, b, c) of each step.  `output` may be `input`.  The products run
  * on the tensor cores: float32 matrices keep fp32 accuracy (two fp16 terms an
- * operand), or that of one TF32 product with DCN_MATH_TF32 in `flags`; 16-bit
- * matrices keep what their type can hold.  A matrix of zeros stays zero for any
- * eps; one with NaN or an infinity gives NaN everywhere.  Made for polynomials that keep singular values of
- * [0, 1] below 2: S is held up to 8, a I + b S + c S S up to 16; beyond, results
- * may be NaN.  At most 32 steps, a of 15 in size and either b and c or the
- * polynomial's values for S in [0, 1] too, 2^31 - 1 elements, a larger side of
- * 2^31 - 256 and a smaller one of 32768. */
+ * operand), or that of one TF32 product with DCN_MATH_TF32 in `flags`; fp16
+ * ones are off by their own rounding; bf16 ones are held in fp16 between the
+ * steps (five usual ones come out 1.7e-3 to 2.0e-3 from the exact answer, 1.66e-3
+ * of it the result's rounding).  A matrix of zeros stays zero for any eps; one
+ * with NaN or an infinity gives NaN everywhere.  Made for polynomials
+ * that keep singular values of [0, 1] below 2: S is held up to 8, a I + b S +
+ * c S S up to 16; beyond, results may be NaN.  At most 32 steps, a of 15 in size
+ * and either b and c or the polynomial's values for S in [0, 1] too, 2^31 - 1
+ * elements, a larger side of 2^31 - 256 and a smaller one of 32768. */
 DCN_API size_t dcn_newton_schulz_workspace_size(int64_t count, int64_t rows, int64_t cols,
                                                 int type, int steps, uint32_t flags);
 DCN_API int dcn_newton_schulz(int64_t count, int64_t rows, int64_t cols, int type,
@@ -382,11 +384,12 @@ DCN_API int dcn_quantize_int8(int64_t rows, int64_t cols, int type, const void* 
  *   output = (sum_k x weight) x_scale[token] weight_scale[channel] + bias,
  * the sum exact.  x is int8 with its scales, or floating (x_scale NULL) and
  * coded as by dcn_quantize_int8 inside the call.  At most 131071 input
- * features, 2^31 - 256 tokens and as many outputs.  Rows of a multiple of 16 features at 16-byte aligned addresses
- * are read where they lie; others are copied first.  Up to 8 tokens of such
- * rows (x and weight aligned) need no workspace: it may be NULL there, and one
- * kernel does it all.  dcn_int8_linear_few_tokens says whether that is also the
- * faster way (1), which a call with a workspace takes by itself. */
+ * features, 2^31 - 256 tokens and as many outputs.  Rows of a multiple of 16
+ * features at 16-byte aligned addresses are read where they lie; others are
+ * copied first.  Up to 8 tokens of such rows (x and weight aligned) need no
+ * workspace: it may be NULL there, and one kernel does it all.
+ * dcn_int8_linear_few_tokens says whether that is also the faster way (1), which
+ * a call with a workspace takes by itself. */
 DCN_API size_t dcn_int8_linear_workspace_size(int64_t tokens, int64_t in_features,
                                               int64_t out_features, int x_type);
 DCN_API int dcn_int8_linear_few_tokens(int64_t tokens, int64_t in_features,

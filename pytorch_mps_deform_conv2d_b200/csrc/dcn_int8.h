@@ -18,8 +18,8 @@ cudaError_t launch_quantize_rows(const void* x, int type, long long rows, int co
                                  signed char* q, long long ldq, float* scale,
                                  cudaStream_t stream);
 // Whether a product of so few tokens can run as one kernel that codes the tokens
-// itself, whether that is the faster way, and that kernel: x (tokens, K) of `x_type` (3: int8 with x_scale),
-// weight (N, K), both dense and 16-byte aligned.
+// itself, whether that is the faster way, and that kernel: x (tokens, K) of
+// `x_type` (3: int8 with x_scale), weight (N, K), both dense and 16-byte aligned.
 bool few_tokens_fit(int64_t tokens, int64_t K);
 bool few_tokens_pay(int x_type, int64_t tokens, int64_t K, int64_t N);
 cudaError_t launch_few_tokens(const void* x, int x_type, const float* x_scale, int tokens, int K,

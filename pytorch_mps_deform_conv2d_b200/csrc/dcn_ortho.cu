@@ -16,10 +16,10 @@
 // three steps of the usual 3.4445, two runs for five steps; results of 16 bits
 // do not see the difference (squarer matrices: run_length below).  For fp32
 // results the first run, where one direction can hold nearly all of |X|, ends
-// before 12: two steps; so does every run of more than 256 directions.  Emulated in 64 bits on 64 x 576 with
-// a few strong directions, the relative error is 5e-7 with runs (2, 3) and
-// 4.6e-6 with (3, 2), fp32 products as written 1.4e-6; one run of five steps
-// diverges on steep spectra.
+// before 12: two steps; so does every run of more than 256 directions.
+// Emulated in 64 bits on 64 x 576 with a few strong directions, the relative
+// error is 5e-7 with runs (2, 3) and 4.6e-6 with (3, 2), fp32 products as
+// written 1.4e-6; one run of five steps diverges on steep spectra.
 #include "dcn_ortho.h"
 
 #include <cmath>
@@ -249,8 +249,8 @@ int run_length(const OrthoShape& s, int first) {
   // The more directions, and the squarer the matrix, the more of them are still
   // small in the second run: up to 256 that run may be long, where the error stays
   // below twice that of fp32 products as written.  From some 350 on it would
-  // pass that, for a twentieth of the time at best.  Relative errors (largest of three gradients
-  // of rank m / 16 under noise), us, with runs (2, 3), with (2, 2, 1), and the
+  // pass that, for a twentieth of the time at best.  Relative errors (largest of
+  // three gradients of rank m / 16 under noise) and us with runs (2, 3), with (2, 2, 1), and the
   // error of fp32 products:
   //   128 x 1152  0.80e-6  79    0.99e-6  90   1.05e-6  (the chain kernel's)
   //   192 x 400   2.2e-6  110    1.7e-6  106   1.6e-6

@@ -499,3 +499,15 @@ def test_two_to_nine_tokens_by_either_way(cuda_device, cin, cout, given):
                                        ws.data_ptr(), None, 0, z.data_ptr(), 0, 0, None, 0,
                                        torch.cuda.current_stream().cuda_stream) == 0
             check_linear(z, q, xs, w, ws, None)
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16], ids=str)
+def test_waits_that_run_out_in_clusters_are_reported(cuda_device, out):
+    # few tiles, K split over a cluster whose partial sums never come
+    dcn.device_status()
+    q, w, s = rand_codes(20, 4096), rand_codes(250, 4096), torch.rand(250, device="cuda")
+    xs = torch.rand(20, device="cuda")
+    _native.load_ops().int8_linear(q, w, s, None, xs, out, TEST_WAIT_TIMEOUT)
+    assert dcn.device_status() & STATUS_DENSE_TIMEOUT
+    check_linear(dcn.int8_linear(q, w, s, x_scale=xs, out_dtype=out), q, xs, w, s, None)
+    dcn.check_device_status()
